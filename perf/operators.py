@@ -70,7 +70,8 @@ def draw(rng) -> dict:
                     drafter=rng.random() < 0.6)
     more = dict(k=_log_int(rng, 1, 256), temperature=rng.choice([0.5, 1.0, 1.0, 2.0, 4.0]), share=rng.choice([0.0, 0.0, 0.5]))
     if kind == "head":
-        return dict(kind=kind, rows=_log_int(rng, 1, 2048), hidden=64 * rng.randint(4, 56), vocab=vocab, **more)
+        # the framework's products want multiples of 8
+        return dict(kind=kind, rows=_log_int(rng, 1, 2048), hidden=64 * rng.randint(4, 56), vocab=vocab // 8 * 8, **more)
     rows = _log_int(rng, 1, min(4096, most // vocab))
     return dict(kind=kind, rows=rows, vocab=vocab, type=rng.choice(["bf16", "bf16", "fp32"]), **more)
 
