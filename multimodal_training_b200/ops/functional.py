@@ -627,3 +627,9 @@ def sum_squares(x: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     else:
         out += x.float().pow(2).sum()
     return out
+
+
+# --------------------------------------------------------------------------------------
+# A second model beside the first: a teacher's top logits, distillation from them, verification of drafts
+# --------------------------------------------------------------------------------------
+from .vocab_rows import distillation_loss, lm_head_distillation, top_logits, verify_drafts  # noqa: E402,F401
