@@ -47,32 +47,35 @@ enum { kTop, kTop1, kSum, kSum1, kDot, kLabel, kStats };
 // ----------------------------------------------------------------------------
 // Teacher's side: one warp per row.  An entry is absent if its id is negative or its logit -inf.
 // ----------------------------------------------------------------------------
-constexpr int kPrepareWarps = 8, kPrepareRows = 32;
+constexpr int kPrepareRows = 8;                    // warps of a block
 template <typename T>
-__global__ void __launch_bounds__(32 * kPrepareWarps) distill_prepare_kernel(const long* ids, long ids_ld, const T* teacher,
+__global__ void __launch_bounds__(32 * kPrepareRows) distill_prepare_kernel(const long* ids, long ids_ld, const T* teacher,
                                                                             long teacher_ld, const long* labels, long rows,
                                                                             long vocab, double inv_temperature,
-                                                                            DistillRows out, long* need,
+                                                                            DistillRows out, long* need, int* ticket,
                                                                             MmtErrorWord* ew) {
   grid_dependency_sync();
-  __shared__ int s_id[kPrepareWarps][kMaxTop];
-  __shared__ double s_p[kPrepareWarps][kMaxTop];
-  __shared__ int n_taught, n_labelled;
+  __shared__ __align__(16) int s_id[kPrepareRows][kMaxTop];
+  __shared__ double s_p[kPrepareRows][kMaxTop];
+  __shared__ int marks[kPrepareRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, K = out.K;
-  if (threadIdx.x == 0) n_taught = n_labelled = 0;
-  __syncthreads();
-  for (int r = warp; r < kPrepareRows; r += kPrepareWarps) {
-    const long row = (long)blockIdx.x * kPrepareRows + r;
-    if (row >= rows) break;
+  const long row = (long)blockIdx.x * kPrepareRows + warp;
+  if (blockIdx.x == 0 && threadIdx.x == 0) ticket[0] = ticket[1] = 0;
+  int mark = 0;
+  if (row < rows) {
     double top = -INFINITY;
     bool any = false, odd = false;                  // odd: a logit that is not a number
-    for (int j = lane; j < K; j += 32) {
-      long id = ids[row * ids_ld + j];
+    for (int j = lane; j < (K + 3) / 4 * 4; j += 32) {
+      long id = -1;
+      float t = -INFINITY;
+      if (j < K) {
+        id = ids[row * ids_ld + j];
+        t = to_float(teacher[row * teacher_ld + j]);
+      }
       if (id >= vocab) {
         mmt_report(ew, MMT_ERR_BOUNDS, 700, (int)row);
         id = -1;
       }
-      const float t = to_float(teacher[row * teacher_ld + j]);
       const bool here = id >= 0 && !(t == -INFINITY);
       s_id[warp][j] = here ? (int)id : -1;
       s_p[warp][j] = here ? (double)t * inv_temperature : -INFINITY;
@@ -82,21 +85,23 @@ __global__ void __launch_bounds__(32 * kPrepareWarps) distill_prepare_kernel(con
     }
     any = __any_sync(0xffffffffu, any);
     odd = __any_sync(0xffffffffu, odd);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (odd) top = NAN;
     double total = 0.0, dot = 0.0;
-    for (int j = lane; j < K; j += 32)
-      if (s_id[warp][j] >= 0) {
-        const double z = s_p[warp][j] - top, e = exp(z);
-        s_p[warp][j] = e;
-        total += e;
-        if (!(e == 0.0)) dot += e * z;
-      }
+    if (any) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      total += __shfl_xor_sync(0xffffffffu, total, o);
-      dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (odd) top = NAN;
+      for (int j = lane; j < K; j += 32)
+        if (s_id[warp][j] >= 0) {
+          const double z = s_p[warp][j] - top, e = exp(z);
+          s_p[warp][j] = e;
+          total += e;
+          if (!(e == 0.0)) dot += e * z;
+        }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+        dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      }
     }
     __syncwarp();
     long label = labels ? labels[row] : -1;
@@ -107,39 +112,56 @@ __global__ void __launch_bounds__(32 * kPrepareWarps) distill_prepare_kernel(con
     // an id that the teacher gives more than once has the sum of its probabilities, in the first of its slots
     double sum_p = 0.0;
     int at_label = K;
+    const double inv_total = any ? 1.0 / total : 0.0;
     for (int j = lane; j < K; j += 32) {
-      const int id = s_id[warp][j];
+      const int id = any ? s_id[warp][j] : -1;
+      float rounded = 0.f;
       bool first = id >= 0;
-      double p = 0.0;
       if (first) {
-        for (int i = 0; i < j; ++i) first &= s_id[warp][i] != id;
-        if (first)
-          for (int i = j; i < K; ++i) p += s_id[warp][i] == id ? s_p[warp][i] : 0.0;
+        int same = 0, before = 0;
+        for (int i = 0; i < K; i += 4) {
+          const int4 q = *reinterpret_cast<const int4*>(&s_id[warp][i]);
+          const int hits = (q.x == id) | (q.y == id) << 1 | (q.z == id) << 2 | (q.w == id) << 3;
+          same += __popc(hits);
+          if (i < j) before |= j - i >= 4 ? hits : hits & ((1 << (j - i)) - 1);
+        }
+        first = before == 0;
+        if (first) {
+          double p = s_p[warp][j];
+          if (same > 1)
+            for (int i = j + 1; i < K; ++i) p += s_id[warp][i] == id ? s_p[warp][i] : 0.0;
+          rounded = (float)(p * inv_total);
+        }
       }
-      const float rounded = first ? (float)(p / total) : 0.f;
       out.slot_id[row * (K + 1) + j] = first ? id : -1;
       out.slot_p[row * (K + 1) + j] = rounded;
       sum_p += (double)rounded;
       if (first && id == label) at_label = j;
     }
+    if (any) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      sum_p += __shfl_xor_sync(0xffffffffu, sum_p, o);
-      at_label = min(at_label, __shfl_xor_sync(0xffffffffu, at_label, o));
+      for (int o = 16; o > 0; o >>= 1) sum_p += __shfl_xor_sync(0xffffffffu, sum_p, o);
     }
+    at_label = __reduce_min_sync(0xffffffffu, at_label);
+    mark = (any ? kTaught : 0) | (label >= 0 ? kLabelled | at_label << kSlotShift : 0);
     if (lane == 0) {
       out.slot_id[row * (K + 1) + K] = label >= 0 && at_label == K ? (int)label : -1;
       out.slot_p[row * (K + 1) + K] = 0.f;
-      out.info[row] = any ? make_double2(dot / total - log(total), sum_p) : make_double2(0.0, 0.0);
-      out.mark[row] = (any ? kTaught : 0) | (label >= 0 ? kLabelled | at_label << kSlotShift : 0);
-      if (need) need[row] = any || label >= 0 ? 0 : -1;
-      if (any) atomicAdd(&n_taught, 1);
-      if (label >= 0) atomicAdd(&n_labelled, 1);
+      out.info[row] = any ? make_double2(dot * inv_total - log(total), sum_p) : make_double2(0.0, 0.0);
+      out.mark[row] = mark;
+      if (need) need[row] = mark ? 0 : -1;
     }
-    __syncwarp();
   }
+  if (lane == 0) marks[warp] = mark;
   __syncthreads();
-  if (threadIdx.x == 0) out.counts[blockIdx.x] = make_int2(n_taught, n_labelled);
+  if (threadIdx.x == 0) {
+    int2 n = make_int2(0, 0);
+    for (int r = 0; r < kPrepareRows; ++r) {
+      n.x += (marks[r] & kTaught) != 0;
+      n.y += (marks[r] & kLabelled) != 0;
+    }
+    out.counts[blockIdx.x] = n;
+  }
 }
 
 // Weights of a row's two gradients, from the number of rows that share them.  `red`: kThreads / 32 values.
@@ -233,17 +255,17 @@ __global__ void __launch_bounds__(kDistillThreads) distill_stats_kernel(const T*
 // ----------------------------------------------------------------------------
 // Gradient from the whole vocabulary's statistics, one CTA per row, into `out` (which may be the logits).
 // ----------------------------------------------------------------------------
-template <typename T, bool kDual>
+template <typename T, typename O, bool kDual>
 __global__ void __launch_bounds__(kDistillThreads) distill_grad_kernel(const T* logits, long ld, int V, long vocab_lo,
                                                                       DistillRows rows, DistillCall call, long n_rows,
                                                                       const long* src, const int* cnt, const double* stats,
-                                                                      const float* dloss, T* out, long out_ld) {
+                                                                      const float* dloss, O* out, long out_ld) {
   grid_dependency_sync();
   __shared__ int red[kDistillThreads / 32];
   __shared__ float slot_x[kMaxTop + 1];
   const Row<T> row(logits + blockIdx.x * ld, V);
-  T* o = out + blockIdx.x * out_ld;
-  const int o_lead = Row<T>::lead_of(o), nv = row.vectors();
+  O* o = out + blockIdx.x * out_ld;
+  const int o_lead = Row<T>::lead_for(o), nv = row.vectors();
   if (cnt) {
     // compacted rows: those behind the last one are not read again, except that the weight gradient's last block of 64
     // rows (the first one if there is none) has to end in zeros
@@ -290,6 +312,243 @@ __global__ void __launch_bounds__(kDistillThreads) distill_grad_kernel(const T* 
     if ((mark & kLabelled) && j == mark >> kSlotShift) g -= wl;
     from_float(g, o + (id - vocab_lo));
   }
+}
+
+// ----------------------------------------------------------------------------
+// Statistics and gradient of a whole vocabulary in one pass over the logits.  A cluster of C CTAs holds one row in shared
+// memory, a run of its vectors each, which a bulk copy brings.  Each CTA reduces its share to (largest, S, S1) and writes
+// that into every CTA of the cluster, and behind one cluster barrier all of them know the row's statistics.  A logit is read
+// once and its gradient written once.
+//
+// Second softmax (kMode): none, or that of temperature one for the labels.  If the temperature is a power of two, its powers
+// are the first one's squared log2(tau) times (c1 = tau c and top1 = tau top exactly).
+//
+// Rows are handed out by tickets: a cluster knows its row and the next one, which is on its way into L2, and takes a ticket
+// for the one after that, which the barrier spreads.  What a CTA is sent for a row is overwritten by the next but one, whose
+// barrier no CTA passes before all have read it.
+// ----------------------------------------------------------------------------
+constexpr int kMaxCluster = 8;
+constexpr int kSingle = 0, kSquares = 1, kTwice = 2;
+
+MMT_DEVICE float pow2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+MMT_DEVICE float thread_max(const uint4& u, float m, bf16) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  __nv_bfloat162 t = *reinterpret_cast<const __nv_bfloat162*>(&w[0]);
+#pragma unroll
+  for (int j = 1; j < 4; ++j) t = __hmax2(t, *reinterpret_cast<const __nv_bfloat162*>(&w[j]));
+  return fmaxf(m, fmaxf(__low2float(t), __high2float(t)));
+}
+MMT_DEVICE float thread_max(const uint4& u, float m, float) {
+  return fmaxf(fmaxf(m, fmaxf(__uint_as_float(u.x), __uint_as_float(u.y))),
+               fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+}
+// Largest of a warp's values, NaN left out.
+MMT_DEVICE float warp_top(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+// 2^(a - b) for two tops, 0 for a set without any mass.
+MMT_DEVICE float rescale(float m, float c, float top) { return m == -INFINITY ? 0.f : pow2(__fmul_rn(m, c) - top); }
+// The two powers of a logit.
+template <int kMode>
+MMT_DEVICE float2 powers(float x, const DistillCall& call, float t, float t1, int squares) {
+  const float e = pow2(__fmaf_rn(x, call.c, -t));
+  float e1 = 0.f;
+  if constexpr (kMode == kTwice) e1 = pow2(__fmaf_rn(x, call.c1, -t1));
+  if constexpr (kMode == kSquares) {
+    e1 = e * e;
+    for (int k = 1; k < squares; ++k) e1 *= e1;
+  }
+  return make_float2(e, e1);
+}
+
+template <typename T, typename O, int kThreads, int kMode>
+__global__ void __launch_bounds__(kThreads, 1280 / kThreads)
+    distill_fused_kernel(const T* logits, long ld, int V, DistillRows rows, DistillCall call, int squares, long n_rows,
+                         int places, const long* src, const int* cnt, double* __restrict__ stats, int* ticket,
+                         const float* dloss, O* out, long out_ld, int per, MmtErrorWord* ew) {
+  grid_dependency_sync();
+  constexpr int kVec = Row<T>::kVec, kWarps = kThreads / 32;
+  constexpr bool kDual = kMode != kSingle;
+  extern __shared__ __align__(128) uint4 held[];   // this CTA's vectors of the row, `per` of them
+  __shared__ uint64_t arrived;
+  __shared__ int red[kWarps];
+  __shared__ float4 warp_part[kWarps];
+  __shared__ float4 cta_part[2][kMaxCluster];
+  __shared__ float2 slots[kMaxTop + 1];            // probability and logit
+  __shared__ int slot_ids[kMaxTop + 1];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int C = (int)cluster_size(), rank = (int)cluster_rank(), clusters = gridDim.x / C;
+  if (tid == 0) {
+    mbar_init(&arrived, 1);
+    mbar_fence_init();
+  }
+  const Weights w = call_weights<kThreads>(rows, call, red);
+  const float d = dloss ? *dloss : 1.f;
+  const float w_taught = (float)(w.taught * (double)call.temperature) * d, w_labelled = (float)w.labelled * d;
+  const int taken = cnt ? *cnt : places;
+  // rows behind the last taken one are not read again, except that the weight gradient's last block of 64 rows (the first
+  // one if there is none) has to end in zeros
+  const int end = cnt ? min(places, max((taken + 63) / 64 * 64, 64)) : places;
+  auto row_at = [&](int place) { return place >= taken ? -1 : src ? (int)src[place] : place; };
+  auto mark_of = [&](int at) { return at < 0 ? 0 : rows.mark[at]; };
+  cluster_barrier();                               // every CTA has started: its shared memory may be written
+  int place = blockIdx.x / C, next = place + clusters;
+  int at = place < end ? row_at(place) : -1, mark = mark_of(at);
+  uint32_t phase = 0;
+  for (int turn = 0; place < end; turn ^= 1) {
+    int after = 0;
+    if (rank == 0 && warp == 0) after = 2 * clusters + (lane == 0 ? atomicAdd(ticket, 1) : 0);
+    const Row<T> row(logits + (long)place * ld, V);
+    const int nv = row.vectors(), first = rank * per, n = max(min(per, nv - first), 0);
+    // [lo, hi): whole vectors of this CTA's run
+    const int lo = min(n, (int)(first == 0 && row.lead != 0)), hi = max(lo, min(n, (row.lead + V) / kVec - first));
+    O* o = out ? out + (long)place * out_ld : nullptr;
+    const int o_lead = Row<T>::lead_for(o);
+    const int next_at = next < end ? row_at(next) : -1, next_mark = mark_of(next_at);
+    if (mark != 0) {
+      if (tid == 0 && lo < hi) {
+        fence_proxy_async_smem();                  // behind what ordinary stores left in `held`
+        mbar_expect_tx(&arrived, (hi - lo) * 16);
+        asm volatile(
+            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                smem_u32(held + lo)),
+            "l"(row.p + row.column(first + lo)), "r"((hi - lo) * 16), "r"(smem_u32(&arrived))
+            : "memory");
+      }
+      if (tid == 32 && next_mark != 0) {
+        const Row<T> ahead(logits + (long)next * ld, V);
+        const int i0 = max(first, (int)(ahead.lead != 0)), i1 = min(first + per, (ahead.lead + V) / kVec);
+        if (i0 < i1)
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(ahead.p + ahead.column(i0)), "r"((i1 - i0) * 16)
+                       : "memory");
+      }
+      if (tid >= 64 && tid < 64 + n - (hi - lo)) {
+        const int i = tid == 64 && lo ? 0 : n - 1;
+        held[i] = row.load(first + i);
+      }
+      for (int j = tid; j <= rows.K; j += kThreads) {
+        const long k = (long)at * (rows.K + 1) + j;
+        const int id = rows.slot_id[k];
+        slots[j] = make_float2(id >= 0 ? rows.slot_p[k] : 0.f, id >= 0 ? to_float(row.p[id]) : 0.f);
+        slot_ids[j] = id;
+      }
+      __syncthreads();
+      if (lo < hi) {
+        mbar_wait(&arrived, phase, ew, 710);
+        phase ^= 1;
+      }
+      float m = -INFINITY;
+#pragma unroll 4
+      for (int i = tid; i < n; i += kThreads) m = thread_max(held[i], m, T());
+      m = warp_top(m);
+      // a warp that has nothing but -inf adds zeros (2^-inf), not 2^(-inf + inf)
+      const float t = m == -INFINITY ? 0.f : __fmul_rn(m, call.c), t1 = m == -INFINITY ? 0.f : __fmul_rn(m, call.c1);
+      float s = 0.f, s1 = 0.f;
+#pragma unroll 2
+      for (int i = tid; i < n; i += kThreads) {
+        float v[kVec];
+        RowVec<T>::unpack(held[i], v);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          const float2 e = powers<kMode>(v[j], call, t, t1, squares);
+          s += e.x;
+          if constexpr (kDual) s1 += e.y;
+        }
+      }
+      s = warp_sum(s);
+      if constexpr (kDual) s1 = warp_sum(s1);
+      if (lane == 0) warp_part[warp] = make_float4(m, s, s1, 0.f);
+      __syncthreads();
+    }
+    if (warp == 0) {
+      after = __shfl_sync(0xffffffffu, after, 0);
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (mark != 0) {
+        a = warp_part[lane % kWarps];
+        const float top = warp_top(a.x);
+        a.y *= rescale(a.x, call.c, __fmul_rn(top, call.c));
+        if constexpr (kDual) a.z *= rescale(a.x, call.c1, __fmul_rn(top, call.c1));
+        a.x = top;
+#pragma unroll
+        for (int k = kWarps / 2; k > 0; k >>= 1) {
+          a.y += __shfl_xor_sync(0xffffffffu, a.y, k);
+          if constexpr (kDual) a.z += __shfl_xor_sync(0xffffffffu, a.z, k);
+        }
+      }
+      a.w = __int_as_float(after);
+      if (lane < C) cluster_store(&cta_part[turn][rank], lane, a);
+    }
+    if (mark == 0 && o) {
+      const float zero[kVec] = {};
+      for (int i = tid; i < n; i += kThreads) row.store(o, o_lead, first + i, zero);
+    }
+    cluster_barrier();
+    after = __float_as_int(cta_part[turn][0].w);
+    if (mark != 0) {
+      // lane k of every warp takes CTA k's part
+      const float4 part = cta_part[turn][lane % C];
+      const float top = warp_top(part.x);
+      const float t = __fmul_rn(top, call.c), t1 = __fmul_rn(top, call.c1);
+      float S = part.y * rescale(part.x, call.c, t), S1 = kDual ? part.z * rescale(part.x, call.c1, t1) : 0.f;
+      for (int k = C / 2; k > 0; k >>= 1) {
+        S += __shfl_xor_sync(0xffffffffu, S, k);
+        if constexpr (kDual) S1 += __shfl_xor_sync(0xffffffffu, S1, k);
+      }
+      const int label_at = mark & kLabelled ? mark >> kSlotShift : -1;
+      if (o) {
+        const float wt = mark & kTaught ? w_taught : 0.f, wl = mark & kLabelled ? w_labelled : 0.f;
+        const float a = (kDual ? wt : wt + wl) / S, a1 = kDual ? wl / S1 : 0.f;
+#pragma unroll 2
+        for (int i = tid; i < n; i += kThreads) {
+          float v[kVec];
+          RowVec<T>::unpack(held[i], v);
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) {
+            const float2 e = powers<kMode>(v[j], call, t, t1, squares);
+            v[j] = kDual ? __fmaf_rn(a, e.x, a1 * e.y) : a * e.x;
+          }
+          row.store(o, o_lead, first + i, v);
+        }
+        __syncthreads();                           // a slot's logit was another thread's
+        for (int j = tid; j <= rows.K; j += kThreads) {
+          const int id = slot_ids[j];
+          if (id < 0 || (unsigned)((id + row.lead) / kVec - first) >= (unsigned)n) continue;
+          const float2 e = powers<kMode>(slots[j].y, call, t, t1, squares);
+          float g = (kDual ? __fmaf_rn(a, e.x, a1 * e.y) : a * e.x) - wt * slots[j].x;
+          if (j == label_at) g -= wl;
+          from_float(g, o + id);
+        }
+      }
+      if (warp == kWarps - 1 && place % C == rank) {
+        double dot = 0.0;
+        for (int j = lane; j <= rows.K; j += 32)
+          if (!(slots[j].x == 0.f)) dot += (double)slots[j].x * (double)slots[j].y;
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, k);
+        if (lane == 0) {
+          stats[kTop * n_rows + at] = t;
+          stats[kTop1 * n_rows + at] = t1;
+          stats[kSum * n_rows + at] = S;
+          stats[kSum1 * n_rows + at] = kDual ? S1 : S;
+          stats[kDot * n_rows + at] = dot;
+          stats[kLabel * n_rows + at] = label_at >= 0 ? (double)slots[label_at].y : 0.0;
+        }
+      }
+      __syncthreads();                             // `held` and `slots` may be written again
+    }
+    place = next;
+    next = after;
+    at = next_at;
+    mark = next_mark;
+  }
+  // the last cluster puts the tickets back for the next launch
+  if (rank == 0 && tid == 0 && atomicAdd(ticket + 1, 1) == clusters - 1) ticket[0] = ticket[1] = 0;
 }
 
 // ----------------------------------------------------------------------------
@@ -356,9 +615,10 @@ struct MmtDistill {
   int* mark;
   int* counts;
   double* stats;
+  int* ticket;                      // two words, zero between launches
   const float* dloss;
   double temperature, share;
-  int V, K, is_f32;
+  int V, K, is_f32, out_f32;
 };
 
 namespace {
@@ -374,7 +634,7 @@ DistillCall call_of(const MmtDistill& d) {
 }
 bool dual(const MmtDistill& d) { return d.share > 0.0 && d.temperature != 1.0; }
 bool wrong(const MmtDistill& d) {
-  return d.K < 1 || d.K > kMaxTop || d.V < 1 || d.rows < 0 || d.places < 0 || d.places > 0x7fffffffL;
+  return d.K < 1 || d.K > kMaxTop || d.V < 1 || d.rows < 0 || d.places < 0 || d.rows > 0x7fffffffL || d.places > 0x7fffffffL;
 }
 
 template <typename T, bool kDual>
@@ -383,11 +643,60 @@ int launch_stats(const MmtDistill& d, void* stream) {
                                reinterpret_cast<const T*>(d.logits), d.ld, d.V, d.vocab_lo, rows_of(d), call_of(d), d.rows,
                                d.src, d.cnt, d.stats);
 }
-template <typename T, bool kDual>
+template <typename T, typename O, bool kDual>
 int launch_grad(const MmtDistill& d, void* stream) {
-  return (int)launch_dependent(distill_grad_kernel<T, kDual>, (unsigned)d.places, kDistillThreads, 0, VR_STREAM(stream),
+  return (int)launch_dependent(distill_grad_kernel<T, O, kDual>, (unsigned)d.places, kDistillThreads, 0, VR_STREAM(stream),
                                reinterpret_cast<const T*>(d.logits), d.ld, d.V, d.vocab_lo, rows_of(d), call_of(d), d.rows,
-                               d.src, d.cnt, d.stats, d.dloss, reinterpret_cast<T*>(d.out), d.out_ld);
+                               d.src, d.cnt, d.stats, d.dloss, reinterpret_cast<O*>(d.out), d.out_ld);
+}
+
+// Vectors that a row has at most, wherever it starts.
+long row_vectors(const MmtDistill& d) {
+  const int vec = d.is_f32 ? 4 : 8;
+  return (d.V + vec - 2) / vec + 1;
+}
+
+constexpr int kHeldBytes = 40 * 1024, kMaxHeldBytes = 200 * 1024;
+
+template <typename T, typename O, int kThreads, int kMode>
+int launch_held(const MmtDistill& d, int C, int per, int squares, void* stream) {
+  auto kernel = distill_fused_kernel<T, O, kThreads, kMode>;
+  static int allowed = 0;
+  const int bytes = per * 16;
+  if (bytes > allowed) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxHeldBytes);
+    if (e != cudaSuccess) return (int)e;
+    allowed = kMaxHeldBytes;
+  }
+  thread_local int known_C = 0, known_bytes = 0, most = 0;
+  if (C != known_C || bytes != known_bytes) {
+    most = resident_clusters(kernel, kThreads, C, bytes);
+    known_C = C;
+    known_bytes = bytes;
+  }
+  const long clusters = d.places < most ? d.places : most;
+  return (int)launch_cluster(kernel, (unsigned)(clusters * C), kThreads, C, bytes, VR_STREAM(stream),
+                             reinterpret_cast<const T*>(d.logits), d.ld, d.V, rows_of(d), call_of(d), squares, d.rows,
+                             (int)d.places, d.src, d.cnt, d.stats, d.ticket, d.dloss, reinterpret_cast<O*>(d.out), d.out_ld,
+                             per, mmt_error_word());
+}
+template <typename T, typename O, int kMode>
+int launch_mode(const MmtDistill& d, int squares, void* stream) {
+  const long nv = row_vectors(d);
+  // as few CTAs a row as hold it in 40 KB each, of which five fit an SM; more where there are few rows
+  int C = 1;
+  while (C < kMaxCluster && nv * 16 > (long)kHeldBytes * C) C *= 2;
+  while (C < kMaxCluster && d.places * C * 2 <= 2 * mmt_sm_count() && nv > 512L * C) C *= 2;
+  const int per = (int)((nv + C - 1) / C);
+  return per * 16 <= kHeldBytes ? launch_held<T, O, 256, kMode>(d, C, per, squares, stream)
+                                : launch_held<T, O, 512, kMode>(d, C, per, squares, stream);
+}
+template <typename T, typename O>
+int launch_fused(const MmtDistill& d, void* stream) {
+  if (!dual(d)) return launch_mode<T, O, kSingle>(d, 0, stream);
+  if (d.temperature == 2.0 || d.temperature == 4.0 || d.temperature == 8.0)
+    return launch_mode<T, O, kSquares>(d, d.temperature == 2.0 ? 1 : d.temperature == 4.0 ? 2 : 3, stream);
+  return launch_mode<T, O, kTwice>(d, 0, stream);
 }
 
 }  // namespace
@@ -408,12 +717,12 @@ int mmt_distill_prepare(const MmtDistill* d, const long* ids, long ids_ld, const
   const unsigned grid = (unsigned)((d->rows + kPrepareRows - 1) / kPrepareRows);
   const double inv = 1.0 / d->temperature;
   if (teacher_f32)
-    return (int)launch_dependent(distill_prepare_kernel<float>, grid, 32 * kPrepareWarps, 0, VR_STREAM(stream), ids, ids_ld,
+    return (int)launch_dependent(distill_prepare_kernel<float>, grid, 32 * kPrepareRows, 0, VR_STREAM(stream), ids, ids_ld,
                                  reinterpret_cast<const float*>(teacher), teacher_ld, labels, d->rows, vocab, inv,
-                                 rows_of(*d), need, mmt_error_word());
-  return (int)launch_dependent(distill_prepare_kernel<bf16>, grid, 32 * kPrepareWarps, 0, VR_STREAM(stream), ids, ids_ld,
+                                 rows_of(*d), need, d->ticket, mmt_error_word());
+  return (int)launch_dependent(distill_prepare_kernel<bf16>, grid, 32 * kPrepareRows, 0, VR_STREAM(stream), ids, ids_ld,
                                reinterpret_cast<const bf16*>(teacher), teacher_ld, labels, d->rows, vocab, inv, rows_of(*d),
-                               need, mmt_error_word());
+                               need, d->ticket, mmt_error_word());
 }
 
 int mmt_distill_stats(const MmtDistill* d, void* stream) {
@@ -424,10 +733,24 @@ int mmt_distill_stats(const MmtDistill* d, void* stream) {
 }
 
 int mmt_distill_grad(const MmtDistill* d, void* stream) {
-  if (wrong(*d)) return -2;
+  if (wrong(*d) || (d->out_f32 && !d->is_f32)) return -2;
   if (d->places == 0) return 0;
-  if (d->is_f32) return dual(*d) ? launch_grad<float, true>(*d, stream) : launch_grad<float, false>(*d, stream);
-  return dual(*d) ? launch_grad<bf16, true>(*d, stream) : launch_grad<bf16, false>(*d, stream);
+  if (d->out_f32) return dual(*d) ? launch_grad<float, float, true>(*d, stream) : launch_grad<float, float, false>(*d, stream);
+  if (d->is_f32) return dual(*d) ? launch_grad<float, bf16, true>(*d, stream) : launch_grad<float, bf16, false>(*d, stream);
+  return dual(*d) ? launch_grad<bf16, bf16, true>(*d, stream) : launch_grad<bf16, bf16, false>(*d, stream);
+}
+
+// Most columns that mmt_distill_fused takes.
+long mmt_distill_fused_columns(int is_f32) {
+  return ((long)kMaxHeldBytes / 16 * kMaxCluster - 1) * (is_f32 ? 4 : 8);
+}
+
+// Statistics of a whole vocabulary and, unless `out` is null, the gradient (times *dloss, if that is not null).
+int mmt_distill_fused(const MmtDistill* d, void* stream) {
+  if (wrong(*d) || (d->out_f32 && !d->is_f32) || d->V > mmt_distill_fused_columns(d->is_f32)) return -2;
+  if (d->places == 0) return 0;
+  if (d->out_f32) return launch_fused<float, float>(*d, stream);
+  return d->is_f32 ? launch_fused<float, bf16>(*d, stream) : launch_fused<bf16, bf16>(*d, stream);
 }
 
 int mmt_distill_loss(const MmtDistill* d, float* loss, void* stream) {

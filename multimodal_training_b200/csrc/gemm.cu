@@ -1950,14 +1950,15 @@ extern "C" int mmt_gemm_bf16(const void* A, const void* B, void* C, const void* 
 // tile that is the best of some bucket is launched; the launches that the count does not belong to return at once.
 // *launches: how many kernels this call has launched.
 extern "C" int mmt_gemm_bf16_counted(const void* A, const void* B, void* C, int M, int N, int K, int lda, int ldb, int ldc,
-                                     int a_mn, int b_mn, int accumulate, const int* cnt, int is_k, int* launches,
-                                     void* stream) {
+                                     int a_mn, int b_mn, int accumulate, int out_f32, const int* cnt, int is_k,
+                                     int* launches, void* stream) {
   *launches = 0;
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   GemmCount c = {cnt, is_k, 1, 0u, 0, 0};
   *launches = 1;
   if (is_k)
-    return gemm_call(A, B, C, nullptr, nullptr, M, N, K, lda, ldb, ldc, 0, a_mn, b_mn, 0, accumulate, 0, 1.f, 0, &c, stream);
+    return gemm_call(A, B, C, nullptr, nullptr, M, N, K, lda, ldb, ldc, 0, a_mn, b_mn, 0, accumulate, out_f32, 1.f, 0, &c,
+                     stream);
   read_env_once();
   const int sms = mmt_sm_count();
   const long kb = (K + BK - 1) / BK;
@@ -1977,8 +1978,8 @@ extern "C" int mmt_gemm_bf16_counted(const void* A, const void* B, void* C, int 
     c.mask = mask[t];
     c.mt = 1 + t / 2;
     c.bn = 192 + 64 * (t & 1);
-    const int rc = gemm_call(A, B, C, nullptr, nullptr, M, N, K, lda, ldb, ldc, 0, a_mn, b_mn, 0, accumulate, 0, 1.f, c.bn,
-                             &c, stream);
+    const int rc = gemm_call(A, B, C, nullptr, nullptr, M, N, K, lda, ldb, ldc, 0, a_mn, b_mn, 0, accumulate, out_f32, 1.f,
+                             c.bn, &c, stream);
     if (rc) return rc;
     ++*launches;
   }

@@ -21,7 +21,8 @@ struct RowVec;
 template <>
 struct RowVec<bf16> {
   static constexpr int kVec = 8;
-  static MMT_DEVICE bf16 none() { return __ushort_as_bfloat16(0xff80); }      // -inf
+  static constexpr uint32_t kNone = 0xff80u;      // -inf
+  static MMT_DEVICE uint32_t bits(bf16 x) { return __bfloat16_as_ushort(x); }
   static MMT_DEVICE void unpack(const uint4& u, float (&v)[8]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -39,7 +40,8 @@ struct RowVec<bf16> {
 template <>
 struct RowVec<float> {
   static constexpr int kVec = 4;
-  static MMT_DEVICE float none() { return -INFINITY; }
+  static constexpr uint32_t kNone = 0xff800000u;
+  static MMT_DEVICE uint32_t bits(float x) { return __float_as_uint(x); }
   static MMT_DEVICE void unpack(const uint4& u, float (&v)[4]) {
     v[0] = __uint_as_float(u.x);
     v[1] = __uint_as_float(u.y);
@@ -67,19 +69,30 @@ struct Row {
   MMT_DEVICE uint4 load(int i) const {
     const int c = column(i);
     if (whole(i)) return *reinterpret_cast<const uint4*>(p + c);
-    alignas(16) T e[kVec];
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-      e[j] = RowVec<T>::none();
-      if (c + j >= 0 && c + j < V) e[j] = p[c + j];
+    // a first or last vector: not unrolled, which costs the others no registers
+    constexpr int kHalf = kVec / 2, kBits = 64 / kHalf;
+    unsigned long long half[2] = {0ull, 0ull};
+#pragma unroll 1
+    for (int j = kVec - 1; j >= 0; --j) {
+      const unsigned long long e = c + j >= 0 && c + j < V ? RowVec<T>::bits(p[c + j]) : RowVec<T>::kNone;
+      if (j >= kHalf) half[1] = half[1] << kBits | e;
+      else half[0] = half[0] << kBits | e;
     }
-    return *reinterpret_cast<const uint4*>(e);
+    return make_uint4((uint32_t)half[0], (uint32_t)(half[0] >> 32), (uint32_t)half[1], (uint32_t)(half[1] >> 32));
   }
-  // Writes the columns of vector i to the row `out`, whose start (`out_lead`) may lie otherwise between two boundaries.
-  MMT_DEVICE void store(T* out, int out_lead, int i, const float (&v)[kVec]) const {
+  // Writes the columns of vector i to the row `out`, of this type or a narrower one, whose start (`out_lead` elements behind
+  // a boundary of kVec of them) may lie otherwise.
+  template <typename O>
+  static MMT_DEVICE int lead_for(const O* out) { return (int)(reinterpret_cast<uintptr_t>(out) / sizeof(O) % kVec); }
+  template <typename O>
+  MMT_DEVICE void store(O* out, int out_lead, int i, const float (&v)[kVec]) const {
     const int c = column(i);
     if (whole(i) && out_lead == lead) {
-      *reinterpret_cast<uint4*>(out + c) = RowVec<T>::pack(v);
+      if constexpr (sizeof(O) == sizeof(T)) {
+        *reinterpret_cast<uint4*>(out + c) = RowVec<T>::pack(v);
+      } else {
+        *reinterpret_cast<uint2*>(out + c) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+      }
       return;
     }
 #pragma unroll
@@ -111,6 +124,74 @@ MMT_DEVICE float block_top(float v, float* red) {
 #pragma unroll
   for (int w = 1; w < kThreads / 32; ++w) t = fmaxf(t, red[w]);
   return t;
+}
+
+// ----------------------------------------------------------------------------
+// Clusters of CTAs that share a row
+// ----------------------------------------------------------------------------
+MMT_DEVICE uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+MMT_DEVICE uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+// All threads of all CTAs of the cluster; shared-memory writes in front of it are seen behind it, in every CTA.
+MMT_DEVICE void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Writes to the place in CTA `rank`'s shared memory that `p` has in this CTA's.
+MMT_DEVICE void cluster_store(float4* p, uint32_t rank, float4 v) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+               : "memory");
+}
+
+// launch_dependent with clusters of `cluster` neighbouring blocks.
+template <typename... Params, typename... Args>
+cudaError_t launch_cluster(void (*kernel)(Params...), dim3 grid, dim3 block, unsigned cluster, size_t smem,
+                           cudaStream_t stream, Args... args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
+// Clusters of a kernel that the current device holds at once.
+template <typename... Params>
+int resident_clusters(void (*kernel)(Params...), unsigned block, unsigned cluster, size_t smem) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cluster);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = mmt_sm_count() / (int)cluster;
+  }
+  return n;
 }
 
 #define VR_STREAM(s) reinterpret_cast<cudaStream_t>(s)

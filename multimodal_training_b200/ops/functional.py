@@ -91,8 +91,8 @@ def _gemm_counted(a, b, out, count: torch.Tensor, *, of_k: bool = False, a_mn: b
         return
     launches = ctypes.c_int()
     nv.call("mmt_gemm_bf16_counted", a.data_ptr(), b.data_ptr(), out.data_ptr(), M, N, K, a.stride(0), b.stride(0),
-            out.stride(0), int(a_mn), int(b_mn), int(accumulate), count.data_ptr(), int(of_k), ctypes.byref(launches),
-            nv.stream())
+            out.stride(0), int(a_mn), int(b_mn), int(accumulate), int(out.dtype == torch.float32), count.data_ptr(),
+            int(of_k), ctypes.byref(launches), nv.stream())
     nv.launch_count += launches.value - 1          # nv.call has counted one
 
 

@@ -147,8 +147,9 @@ class _DistillWords(ctypes.Structure):
                 ("vocab_lo", ctypes.c_long), ("rows", ctypes.c_long), ("places", ctypes.c_long), ("src", ctypes.c_void_p),
                 ("cnt", ctypes.c_void_p), ("slot_id", ctypes.c_void_p), ("slot_p", ctypes.c_void_p),
                 ("info", ctypes.c_void_p), ("mark", ctypes.c_void_p), ("counts", ctypes.c_void_p),
-                ("stats", ctypes.c_void_p), ("dloss", ctypes.c_void_p), ("temperature", ctypes.c_double),
-                ("share", ctypes.c_double), ("V", ctypes.c_int), ("K", ctypes.c_int), ("is_f32", ctypes.c_int)]
+                ("stats", ctypes.c_void_p), ("ticket", ctypes.c_void_p), ("dloss", ctypes.c_void_p),
+                ("temperature", ctypes.c_double), ("share", ctypes.c_double), ("V", ctypes.c_int), ("K", ctypes.c_int), ("is_f32", ctypes.c_int),
+                ("out_f32", ctypes.c_int)]
 
 
 nv.declare("mmt_distill_bytes", nv.c_int, [])
@@ -157,6 +158,8 @@ nv.declare("mmt_distill_prepare", nv.c_int, [nv._P, nv._P, nv.c_long, nv._P, nv.
                                              nv._P])
 nv.declare("mmt_distill_stats", nv.c_int, [nv._P, nv._P])
 nv.declare("mmt_distill_grad", nv.c_int, [nv._P, nv._P])
+nv.declare("mmt_distill_fused", nv.c_int, [nv._P, nv._P])
+nv.declare("mmt_distill_fused_columns", nv.c_long, [nv.c_int])
 nv.declare("mmt_distill_loss", nv.c_int, [nv._P, nv._P, nv._P])
 nv.declare("mmt_distill_scale", nv.c_int, [nv._P, nv.c_int, nv.c_long, nv._P, nv._P])
 
@@ -182,6 +185,7 @@ class _Distill:
         w.slot_id = at + 8 * n_counts
         w.slot_p = w.slot_id + 4 * rows * (K + 1)
         w.mark = w.slot_p + 4 * rows * (K + 1)
+        w.ticket = w.mark + 4 * rows
         if rows:
             nv.call("mmt_distill_prepare", ctypes.addressof(w), teacher_ids.data_ptr(), _ld(teacher_ids),
                     teacher_logits.data_ptr(), _ld(teacher_logits), int(teacher_logits.dtype == torch.float32),
@@ -213,10 +217,28 @@ class _Distill:
         self.stats[:2, lo:hi] = top
         self.stats[2:, lo:hi] = rest
 
+    def _out(self, out, dloss=None) -> None:
+        w = self.words
+        w.out, w.out_ld, w.dloss = nv.ptr(out), 0 if out is None else _ld(out), nv.ptr(dloss)
+        w.out_f32 = int(out is not None and out.dtype == torch.float32)
+
+    def both(self, logits, out, src=None, cnt=None, dloss=None) -> None:
+        """Statistics of a whole vocabulary and (unless ``out`` is None) the gradient."""
+        w = self.words
+        if w.V > nv.lib().mmt_distill_fused_columns(w.is_f32):
+            self.row_stats(logits, src, cnt)
+            if out is not None:
+                self.grad(logits, out, src, cnt, dloss)
+            return
+        self._rows(logits, src, cnt)
+        self._out(out, dloss)
+        if logits.shape[0]:
+            nv.call("mmt_distill_fused", ctypes.addressof(w), nv.stream())
+
     def grad(self, logits, out, src=None, cnt=None, dloss=None) -> None:
         self._rows(logits, src, cnt)
+        self._out(out, dloss)
         w = self.words
-        w.out, w.out_ld, w.dloss = out.data_ptr(), _ld(out), nv.ptr(dloss)
         if logits.shape[0]:
             nv.call("mmt_distill_grad", ctypes.addressof(w), nv.stream())
 
@@ -229,7 +251,7 @@ class _Distill:
 class _DistillFn(torch.autograd.Function):
     """The gradient is written in forward, while the row's statistics are at hand, and handed over by the first backward
     pass (times its ``dloss``, where that is not one).  Another backward pass, and one that is captured into a graph (a
-    replay would scale once more), form it again from the logits and the statistics."""
+    replay would scale once more), form it again from the logits."""
 
     @staticmethod
     def forward(ctx, logits, teacher_ids, teacher_logits, labels, temperature, share, vocab_lo, group):
@@ -237,16 +259,19 @@ class _DistillFn(torch.autograd.Function):
         world = torch.distributed.get_world_size(group) if _multi(group) else 1
         d = _Distill(teacher_ids, teacher_logits, labels, temperature, share, vocab_lo, V * world,
                      logits.dtype == torch.float32, V)
-        d.row_stats(logits)
-        if world > 1:
-            d.reduce(0, rows, group)
         ctx.early = None
         if ctx.needs_input_grad[0]:
             if not torch.cuda.is_current_stream_capturing():
                 ctx.early = torch.empty(rows, V, device=logits.device, dtype=logits.dtype)
-                d.grad(logits, ctx.early)
             ctx.save_for_backward(logits, *d.tensors())
-            ctx.d = d
+            ctx.d, ctx.world = d, world
+        if world > 1:
+            d.row_stats(logits)
+            d.reduce(0, rows, group)
+            if ctx.early is not None:
+                d.grad(logits, ctx.early)
+        else:
+            d.both(logits, ctx.early)
         return d.loss()
 
     @staticmethod
@@ -261,7 +286,7 @@ class _DistillFn(torch.autograd.Function):
         else:
             logits = ctx.saved_tensors[0]
             grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-            ctx.d.grad(logits, grad, dloss=dloss)
+            (ctx.d.grad if ctx.world > 1 else ctx.d.both)(logits, grad, dloss=dloss)
         return (grad,) + (None,) * 7
 
 
@@ -373,14 +398,16 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
 def _head_pass(hidden, weight, teacher, temperature, share, vocab_lo, group, chunk_rows, need_h, dw, add):
     """Loss, and the gradient of ``hidden`` (if ``need_h``) and of ``weight`` (into ``dw``, on top of it if ``add``).
 
-    As the head's cross-entropy: the logits of a chunk of rows live in a bf16 workspace only and their gradient replaces
-    them there.  Rows without a teacher or label are left out of the products in groups of 16."""
+    As in the head's cross-entropy, the logits of a chunk of rows and their gradient live in workspaces only, and rows
+    without a teacher or label are left out of the products in groups of 16.  The logits stay fp32: rounded to bf16 they
+    would move a row's loss by 2^-9 of their size, where the divergence is what is left of numbers of that size.  Their
+    gradient is rounded to bf16 once, for the tensor cores."""
     from . import functional as F
     T, V = hidden.shape[0], weight.shape[0]
     dev = hidden.device
     world = torch.distributed.get_world_size(group) if _multi(group) else 1
     need = torch.empty(T, device=dev, dtype=torch.int64)
-    d = _Distill(*teacher, temperature, share, vocab_lo, V * world, False, V, need)
+    d = _Distill(*teacher, temperature, share, vocab_lo, V * world, True, V, need)
     if T == 0:
         if dw is not None and not add:
             dw.zero_()
@@ -392,21 +419,24 @@ def _head_pass(hidden, weight, teacher, temperature, share, vocab_lo, group, chu
             count.data_ptr(), nv.stream())
     x = F.gather_rows_raw(hidden, src)
     dx = torch.empty_like(hidden) if need_h else None
-    ws = torch.empty(chunk_rows, V, device=dev, dtype=torch.bfloat16)
+    ws = torch.empty(chunk_rows, V, device=dev, dtype=torch.float32)
+    gs = torch.empty(chunk_rows, V, device=dev, dtype=torch.bfloat16) if need_h or dw is not None else None
     for i, c0 in enumerate(range(0, T, chunk_rows)):
         c1 = min(T, c0 + chunk_rows)
         h, logits, n = x[c0:c1], ws[:c1 - c0], count[i:]
+        grad = None if gs is None else gs[:c1 - c0]
         F._gemm_counted(h, weight, logits, n)
-        d.row_stats(logits, src[c0:], n)
         if world > 1:
+            d.row_stats(logits, src[c0:], n)
             d.reduce(c0, c1, group)
-        if not need_h and dw is None:
-            continue
-        d.grad(logits, logits, src[c0:], n)
+            if grad is not None:
+                d.grad(logits, grad, src[c0:], n)
+        else:
+            d.both(logits, grad, src[c0:], n)
         if need_h:
-            F._gemm_counted(logits, weight, dx[c0:c1], n, b_mn=True)
+            F._gemm_counted(grad, weight, dx[c0:c1], n, b_mn=True)
         if dw is not None:
-            F._gemm_counted(logits, h, dw, n, of_k=True, a_mn=True, b_mn=True, accumulate=add or c0 > 0)
+            F._gemm_counted(grad, h, dw, n, of_k=True, a_mn=True, b_mn=True, accumulate=add or c0 > 0)
     return d.loss(), F.gather_rows_raw(dx, pos) if need_h else None
 
 
@@ -461,8 +491,8 @@ def lm_head_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids
     """:func:`distillation_loss` of ``hidden @ weight^T`` without keeping the logits: ``hidden`` is [T, H], ``weight`` this
     rank's [V_local, H] shard of the head, teacher and labels are those of the T rows.
 
-    On the GPU path the logits are rounded to bf16, as those of :func:`.functional.lm_head_cross_entropy` are, and the
-    weight gradient assumes ``dloss == 1`` when it is written into ``main_grad``; H and V_local are multiples of 8.
+    On the GPU path hidden states and weight are bf16, H and V_local multiples of 8, and the weight gradient assumes
+    ``dloss == 1`` when it is written into ``main_grad``, as in :func:`.functional.lm_head_cross_entropy`.
     """
     if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
         raise ValueError(f"hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} must be [T, H] and [V, H]")
