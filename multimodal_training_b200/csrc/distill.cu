@@ -323,9 +323,12 @@ __global__ void __launch_bounds__(kDistillThreads) distill_grad_kernel(const T* 
 // Second softmax (kMode): none, or that of temperature one for the labels.  If the temperature is a power of two, its powers
 // are the first one's squared log2(tau) times (c1 = tau c and top1 = tau top exactly).
 //
+// The parts travel as asynchronous stores that count themselves into an mbarrier of the CTA they go to (two of them, in
+// turn: a CTA may be a row ahead of another, never two).  A barrier of the cluster would also wait until the gradients that
+// the threads have stored are visible, which is several microseconds.
+//
 // Rows are handed out by tickets: a cluster knows its row and the next one, which is on its way into L2, and takes a ticket
-// for the one after that, which the barrier spreads.  What a CTA is sent for a row is overwritten by the next but one, whose
-// barrier no CTA passes before all have read it.
+// for the one after that, which travels with the parts.
 // ----------------------------------------------------------------------------
 constexpr int kMaxCluster = 8;
 constexpr int kSingle = 0, kSquares = 1, kTwice = 2;
@@ -376,16 +379,18 @@ __global__ void __launch_bounds__(kThreads, 1280 / kThreads)
   constexpr int kVec = Row<T>::kVec, kWarps = kThreads / 32;
   constexpr bool kDual = kMode != kSingle;
   extern __shared__ __align__(128) uint4 held[];   // this CTA's vectors of the row, `per` of them
-  __shared__ uint64_t arrived;
+  __shared__ uint64_t arrived, met[2];
   __shared__ int red[kWarps];
   __shared__ float4 warp_part[kWarps];
   __shared__ float4 cta_part[2][kMaxCluster];
-  __shared__ float2 slots[kMaxTop + 1];            // probability and logit
-  __shared__ int slot_ids[kMaxTop + 1];
+  __shared__ float2 slots[2][kMaxTop + 1];         // probability and logit
+  __shared__ int slot_ids[2][kMaxTop + 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int C = (int)cluster_size(), rank = (int)cluster_rank(), clusters = gridDim.x / C;
+  const int C = (int)cluster_size(), rank = (int)cluster_rank(), clusters = gridDim.x / C, first = rank * per;
   if (tid == 0) {
     mbar_init(&arrived, 1);
+    mbar_init(&met[0], 1);
+    mbar_init(&met[1], 1);
     mbar_fence_init();
   }
   const Weights w = call_weights<kThreads>(rows, call, red);
@@ -397,52 +402,63 @@ __global__ void __launch_bounds__(kThreads, 1280 / kThreads)
   const int end = cnt ? min(places, max((taken + 63) / 64 * 64, 64)) : places;
   auto row_at = [&](int place) { return place >= taken ? -1 : src ? (int)src[place] : place; };
   auto mark_of = [&](int at) { return at < 0 ? 0 : rows.mark[at]; };
+  auto row_of = [&](int place) { return Row<T>(logits + (long)place * ld, V); };
+  // Whole vectors of this CTA's run of a row, from the run's first.
+  auto whole = [&](const Row<T>& row, int n) {
+    const int lo = min(n, (int)(first == 0 && row.lead != 0));
+    return make_int2(lo, max(lo, min(n, (row.lead + V) / kVec - first)));
+  };
+  auto fetch = [&](int place) {
+    const Row<T> row = row_of(place);
+    const int2 r = whole(row, max(min(per, row.vectors() - first), 0));
+    if (r.x >= r.y) return;
+    fence_proxy_async_smem();                      // behind what ordinary stores left in `held`
+    mbar_expect_tx(&arrived, (r.y - r.x) * 16);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(held + r.x)),
+                 "l"(row.p + row.column(first + r.x)), "r"((r.y - r.x) * 16), "r"(smem_u32(&arrived))
+                 : "memory");
+  };
   cluster_barrier();                               // every CTA has started: its shared memory may be written
   int place = blockIdx.x / C, next = place + clusters;
   int at = place < end ? row_at(place) : -1, mark = mark_of(at);
+  if (tid == 0 && mark != 0) fetch(place);
   uint32_t phase = 0;
-  for (int turn = 0; place < end; turn ^= 1) {
+  for (int k = 0; place < end; ++k) {
+    const int turn = k & 1;
     int after = 0;
     if (rank == 0 && warp == 0) after = 2 * clusters + (lane == 0 ? atomicAdd(ticket, 1) : 0);
-    const Row<T> row(logits + (long)place * ld, V);
-    const int nv = row.vectors(), first = rank * per, n = max(min(per, nv - first), 0);
-    // [lo, hi): whole vectors of this CTA's run
-    const int lo = min(n, (int)(first == 0 && row.lead != 0)), hi = max(lo, min(n, (row.lead + V) / kVec - first));
+    const Row<T> row = row_of(place);
+    const int n = max(min(per, row.vectors() - first), 0);
+    const int2 mid = whole(row, n);
     O* o = out ? out + (long)place * out_ld : nullptr;
     const int o_lead = Row<T>::lead_for(o);
     const int next_at = next < end ? row_at(next) : -1, next_mark = mark_of(next_at);
     if (mark != 0) {
-      if (tid == 0 && lo < hi) {
-        fence_proxy_async_smem();                  // behind what ordinary stores left in `held`
-        mbar_expect_tx(&arrived, (hi - lo) * 16);
-        asm volatile(
-            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                smem_u32(held + lo)),
-            "l"(row.p + row.column(first + lo)), "r"((hi - lo) * 16), "r"(smem_u32(&arrived))
-            : "memory");
-      }
       if (tid == 32 && next_mark != 0) {
-        const Row<T> ahead(logits + (long)next * ld, V);
-        const int i0 = max(first, (int)(ahead.lead != 0)), i1 = min(first + per, (ahead.lead + V) / kVec);
-        if (i0 < i1)
-          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(ahead.p + ahead.column(i0)), "r"((i1 - i0) * 16)
+        const Row<T> ahead = row_of(next);
+        const int2 r = whole(ahead, max(min(per, ahead.vectors() - first), 0));
+        if (r.x < r.y)
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(ahead.p + ahead.column(first + r.x)),
+                       "r"((r.y - r.x) * 16)
                        : "memory");
       }
-      if (tid >= 64 && tid < 64 + n - (hi - lo)) {
-        const int i = tid == 64 && lo ? 0 : n - 1;
+      if (tid >= 64 && tid < 64 + n - (mid.y - mid.x)) {
+        const int i = tid == 64 && mid.x ? 0 : n - 1;
         held[i] = row.load(first + i);
       }
       for (int j = tid; j <= rows.K; j += kThreads) {
-        const long k = (long)at * (rows.K + 1) + j;
-        const int id = rows.slot_id[k];
-        slots[j] = make_float2(id >= 0 ? rows.slot_p[k] : 0.f, id >= 0 ? to_float(row.p[id]) : 0.f);
-        slot_ids[j] = id;
+        const long q = (long)at * (rows.K + 1) + j;
+        const int id = rows.slot_id[q];
+        slots[turn][j] = make_float2(id >= 0 ? rows.slot_p[q] : 0.f, id >= 0 ? to_float(row.p[id]) : 0.f);
+        slot_ids[turn][j] = id;
       }
-      __syncthreads();
-      if (lo < hi) {
-        mbar_wait(&arrived, phase, ew, 710);
+      // one warp waits for the copy, the others without issuing anything at the barrier
+      if (mid.x < mid.y) {
+        if (warp == 0) mbar_wait(&arrived, phase, ew, 710);
         phase ^= 1;
       }
+      __syncthreads();
       float m = -INFINITY;
 #pragma unroll 4
       for (int i = tid; i < n; i += kThreads) m = thread_max(held[i], m, T());
@@ -476,71 +492,89 @@ __global__ void __launch_bounds__(kThreads, 1280 / kThreads)
         if constexpr (kDual) a.z *= rescale(a.x, call.c1, __fmul_rn(top, call.c1));
         a.x = top;
 #pragma unroll
-        for (int k = kWarps / 2; k > 0; k >>= 1) {
-          a.y += __shfl_xor_sync(0xffffffffu, a.y, k);
-          if constexpr (kDual) a.z += __shfl_xor_sync(0xffffffffu, a.z, k);
+        for (int q = kWarps / 2; q > 0; q >>= 1) {
+          a.y += __shfl_xor_sync(0xffffffffu, a.y, q);
+          if constexpr (kDual) a.z += __shfl_xor_sync(0xffffffffu, a.z, q);
         }
       }
       a.w = __int_as_float(after);
-      if (lane < C) cluster_store(&cta_part[turn][rank], lane, a);
+      if (lane == 0) mbar_expect_tx(&met[turn], C * 16);
+      __syncwarp();
+      if (lane < C) cluster_send(&cta_part[turn][rank], &met[turn], lane, a);
     }
     if (mark == 0 && o) {
       const float zero[kVec] = {};
       for (int i = tid; i < n; i += kThreads) row.store(o, o_lead, first + i, zero);
     }
-    cluster_barrier();
+    if (warp == 0) cluster_wait(&met[turn], k >> 1 & 1, ew, 711);
+    __syncthreads();
     after = __float_as_int(cta_part[turn][0].w);
     if (mark != 0) {
-      // lane k of every warp takes CTA k's part
+      // lane q of every warp takes CTA q's part
       const float4 part = cta_part[turn][lane % C];
       const float top = warp_top(part.x);
       const float t = __fmul_rn(top, call.c), t1 = __fmul_rn(top, call.c1);
       float S = part.y * rescale(part.x, call.c, t), S1 = kDual ? part.z * rescale(part.x, call.c1, t1) : 0.f;
-      for (int k = C / 2; k > 0; k >>= 1) {
-        S += __shfl_xor_sync(0xffffffffu, S, k);
-        if constexpr (kDual) S1 += __shfl_xor_sync(0xffffffffu, S1, k);
+      for (int q = C / 2; q > 0; q >>= 1) {
+        S += __shfl_xor_sync(0xffffffffu, S, q);
+        if constexpr (kDual) S1 += __shfl_xor_sync(0xffffffffu, S1, q);
       }
       const int label_at = mark & kLabelled ? mark >> kSlotShift : -1;
+      const float wt = mark & kTaught ? w_taught : 0.f, wl = mark & kLabelled ? w_labelled : 0.f;
+      const float a = (kDual ? wt : wt + wl) / S, a1 = kDual ? wl / S1 : 0.f;
+      auto grad = [&](float x) {
+        const float2 e = powers<kMode>(x, call, t, t1, squares);
+        return kDual ? __fmaf_rn(a, e.x, a1 * e.y) : a * e.x;
+      };
       if (o) {
-        const float wt = mark & kTaught ? w_taught : 0.f, wl = mark & kLabelled ? w_labelled : 0.f;
-        const float a = (kDual ? wt : wt + wl) / S, a1 = kDual ? wl / S1 : 0.f;
+        const bool in_step = o_lead == row.lead;   // whole vectors may be stored whole
+        const int lo = in_step ? mid.x : 0, hi = in_step ? mid.y : n;
 #pragma unroll 2
-        for (int i = tid; i < n; i += kThreads) {
+        for (int i = lo + tid; i < hi; i += kThreads) {
           float v[kVec];
           RowVec<T>::unpack(held[i], v);
 #pragma unroll
-          for (int j = 0; j < kVec; ++j) {
-            const float2 e = powers<kMode>(v[j], call, t, t1, squares);
-            v[j] = kDual ? __fmaf_rn(a, e.x, a1 * e.y) : a * e.x;
-          }
+          for (int j = 0; j < kVec; ++j) v[j] = grad(v[j]);
+          if (in_step) Row<T>::store_whole(o + row.column(first + i), v);
+          else row.store(o, o_lead, first + i, v);
+        }
+        if (tid >= kThreads - n + (hi - lo)) {     // the others
+          const int i = tid == kThreads - 1 && lo ? 0 : n - 1;
+          float v[kVec];
+          RowVec<T>::unpack(held[i], v);
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) v[j] = grad(v[j]);
           row.store(o, o_lead, first + i, v);
         }
-        __syncthreads();                           // a slot's logit was another thread's
+      }
+      __syncthreads();                             // `held` may be written again; a slot's logit was another thread's
+      if (tid == 0 && next_mark != 0) fetch(next);
+      if (o)
         for (int j = tid; j <= rows.K; j += kThreads) {
-          const int id = slot_ids[j];
+          const int id = slot_ids[turn][j];
           if (id < 0 || (unsigned)((id + row.lead) / kVec - first) >= (unsigned)n) continue;
-          const float2 e = powers<kMode>(slots[j].y, call, t, t1, squares);
-          float g = (kDual ? __fmaf_rn(a, e.x, a1 * e.y) : a * e.x) - wt * slots[j].x;
+          float g = grad(slots[turn][j].y) - wt * slots[turn][j].x;
           if (j == label_at) g -= wl;
           from_float(g, o + id);
         }
-      }
       if (warp == kWarps - 1 && place % C == rank) {
         double dot = 0.0;
         for (int j = lane; j <= rows.K; j += 32)
-          if (!(slots[j].x == 0.f)) dot += (double)slots[j].x * (double)slots[j].y;
+          if (!(slots[turn][j].x == 0.f)) dot += (double)slots[turn][j].x * (double)slots[turn][j].y;
 #pragma unroll
-        for (int k = 16; k > 0; k >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, k);
+        for (int q = 16; q > 0; q >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, q);
         if (lane == 0) {
           stats[kTop * n_rows + at] = t;
           stats[kTop1 * n_rows + at] = t1;
           stats[kSum * n_rows + at] = S;
           stats[kSum1 * n_rows + at] = kDual ? S1 : S;
           stats[kDot * n_rows + at] = dot;
-          stats[kLabel * n_rows + at] = label_at >= 0 ? (double)slots[label_at].y : 0.0;
+          stats[kLabel * n_rows + at] = label_at >= 0 ? (double)slots[turn][label_at].y : 0.0;
         }
       }
-      __syncthreads();                             // `held` and `slots` may be written again
+    } else {
+      __syncthreads();                             // all have read the ticket
+      if (tid == 0 && next_mark != 0) fetch(next);
     }
     place = next;
     next = after;

@@ -85,14 +85,15 @@ struct Row {
   template <typename O>
   static MMT_DEVICE int lead_for(const O* out) { return (int)(reinterpret_cast<uintptr_t>(out) / sizeof(O) % kVec); }
   template <typename O>
+  static MMT_DEVICE void store_whole(O* to, const float (&v)[kVec]) {
+    if constexpr (sizeof(O) == sizeof(T)) *reinterpret_cast<uint4*>(to) = RowVec<T>::pack(v);
+    else *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+  }
+  template <typename O>
   MMT_DEVICE void store(O* out, int out_lead, int i, const float (&v)[kVec]) const {
     const int c = column(i);
     if (whole(i) && out_lead == lead) {
-      if constexpr (sizeof(O) == sizeof(T)) {
-        *reinterpret_cast<uint4*>(out + c) = RowVec<T>::pack(v);
-      } else {
-        *reinterpret_cast<uint2*>(out + c) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-      }
+      store_whole(out + c, v);
       return;
     }
 #pragma unroll
@@ -143,12 +144,42 @@ MMT_DEVICE uint32_t cluster_size() {
 MMT_DEVICE void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Writes to the place in CTA `rank`'s shared memory that `p` has in this CTA's.
-MMT_DEVICE void cluster_store(float4* p, uint32_t rank, float4 v) {
-  uint32_t a;
+// Writes to the place in CTA `rank`'s shared memory that `p` has in this CTA's, and counts the 16 bytes into the mbarrier
+// there that `bar` is here.
+MMT_DEVICE void cluster_send(float4* p, uint64_t* bar, uint32_t rank, float4 v) {
+  uint32_t a, b;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(smem_u32(bar)), "r"(rank));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(a),
+               "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(b)
                : "memory");
+}
+
+// mbar_wait (common.cuh) for what other CTAs of the cluster have sent.
+MMT_DEVICE bool cluster_wait(uint64_t* bar, uint32_t parity, MmtErrorWord* ew, int where) {
+  const uint32_t addr = smem_u32(bar);
+  uint64_t t0 = 0;
+  for (uint32_t it = 0;; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t"
+        "}\n"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((it & 0x3ff) == 0x3ff) {
+      const uint64_t now = mmt_globaltimer();
+      if (t0 == 0) t0 = now;
+      else if (now - t0 > MMT_WAIT_NS) {
+        mmt_report(ew, MMT_ERR_MBAR_TIMEOUT, where, (int)parity);
+        return false;
+      }
+    }
+  }
 }
 
 // launch_dependent with clusters of `cluster` neighbouring blocks.
