@@ -40,9 +40,10 @@ struct DistillCall {
   float temperature, share;
 };
 
-// Per row, in statistics of [6][rows]: top and top1 = fl(max x * c1), S and S1, sum of p x over the slots of this shard,
-// the label's logit if it is in this shard.
-enum { kTop, kTop1, kSum, kSum1, kDot, kLabel, kStats };
+// Per row, in statistics of [kStats][rows]: top and top1 = fl(max x * c1), S and S1, the label's logit if it is in this
+// shard, sum of p x over the slots of this shard.  Or parts of the row's loss, one from each CTA that has worked on it.
+constexpr int kMaxCluster = 8;
+enum { kTop, kTop1, kSum, kSum1, kLabel, kDot, kStats = kMaxCluster };
 
 // ----------------------------------------------------------------------------
 // Teacher's side: one warp per row.  An entry is absent if its id is negative or its logit -inf.
@@ -52,7 +53,8 @@ template <typename T>
 __global__ void __launch_bounds__(32 * kPrepareRows) distill_prepare_kernel(const long* ids, long ids_ld, const T* teacher,
                                                                             long teacher_ld, const long* labels, long rows,
                                                                             long vocab, double inv_temperature,
-                                                                            DistillRows out, long* need, int* ticket,
+                                                                            DistillRows out, long* need,
+                                                                            double* stats, int* ticket,
                                                                             MmtErrorWord* ew) {
   grid_dependency_sync();
   __shared__ __align__(16) int s_id[kPrepareRows][kMaxTop];
@@ -152,6 +154,7 @@ __global__ void __launch_bounds__(32 * kPrepareRows) distill_prepare_kernel(cons
       if (need) need[row] = mark ? 0 : -1;
     }
   }
+  if (row < rows && mark == 0 && lane < kStats) stats[lane * rows + row] = 0.0;      // such a row has no loss
   if (lane == 0) marks[warp] = mark;
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -198,7 +201,7 @@ __global__ void __launch_bounds__(kDistillThreads) distill_stats_kernel(const T*
   if (at < 0) return;
   const int mark = rows.mark[at];
   if (mark == 0) {
-    if (threadIdx.x < kStats) stats[threadIdx.x * n_rows + at] = threadIdx.x == kSum || threadIdx.x == kSum1 ? 1.0 : 0.0;
+    if (threadIdx.x <= kDot) stats[threadIdx.x * n_rows + at] = threadIdx.x == kSum || threadIdx.x == kSum1 ? 1.0 : 0.0;
     return;
   }
   const Row<T> row(logits + blockIdx.x * ld, V);
@@ -330,7 +333,6 @@ __global__ void __launch_bounds__(kDistillThreads) distill_grad_kernel(const T* 
 // Rows are handed out by tickets: a cluster knows its row and the next one, which is on its way into L2, and takes a ticket
 // for the one after that, which travels with the parts.
 // ----------------------------------------------------------------------------
-constexpr int kMaxCluster = 8;
 constexpr int kSingle = 0, kSquares = 1, kTwice = 2;
 
 MMT_DEVICE float pow2(float x) {
@@ -357,18 +359,54 @@ MMT_DEVICE float warp_top(float v) {
 }
 // 2^(a - b) for two tops, 0 for a set without any mass.
 MMT_DEVICE float rescale(float m, float c, float top) { return m == -INFINITY ? 0.f : pow2(__fmul_rn(m, c) - top); }
-// The two powers of a logit.
-template <int kMode>
-MMT_DEVICE float2 powers(float x, const DistillCall& call, float t, float t1, int squares) {
-  const float e = pow2(__fmaf_rn(x, call.c, -t));
-  float e1 = 0.f;
-  if constexpr (kMode == kTwice) e1 = pow2(__fmaf_rn(x, call.c1, -t1));
-  if constexpr (kMode == kSquares) {
-    e1 = e * e;
-    for (int k = 1; k < squares; ++k) e1 *= e1;
-  }
-  return make_float2(e, e1);
+
+// Two fp32 values in one 64-bit register: an instruction works on both.
+typedef unsigned long long f32x2;
+MMT_DEVICE f32x2 both(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
 }
+MMT_DEVICE float2 apart(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+MMT_DEVICE f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+MMT_DEVICE f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+MMT_DEVICE f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// The two powers of two logits, with c = (c, c) and so on.
+struct Powers {
+  f32x2 c, c1, less, less1;               // less = (-top, -top)
+  int squares;
+  MMT_DEVICE Powers(const DistillCall& call, float t, float t1, int squares_)
+      : c(both(call.c, call.c)), c1(both(call.c1, call.c1)), less(both(-t, -t)), less1(both(-t1, -t1)), squares(squares_) {}
+  template <int kMode>
+  MMT_DEVICE void take(f32x2 x, f32x2& e, f32x2& e1) const {
+    float2 v = apart(fma2(x, c, less));
+    e = both(pow2(v.x), pow2(v.y));
+    if constexpr (kMode == kTwice) {
+      v = apart(fma2(x, c1, less1));
+      e1 = both(pow2(v.x), pow2(v.y));
+    }
+    if constexpr (kMode == kSquares) {
+      e1 = mul2(e, e);
+      for (int k = 1; k < squares; ++k) e1 = mul2(e1, e1);
+    }
+  }
+};
 
 template <typename T, typename O, int kThreads, int kMode>
 __global__ void __launch_bounds__(kThreads, 1280 / kThreads)
@@ -383,8 +421,8 @@ __global__ void __launch_bounds__(kThreads, 1280 / kThreads)
   __shared__ int red[kWarps];
   __shared__ float4 warp_part[kWarps];
   __shared__ float4 cta_part[2][kMaxCluster];
-  __shared__ float2 slots[2][kMaxTop + 1];         // probability and logit
   __shared__ int slot_ids[2][kMaxTop + 1];
+  __shared__ float slot_ps[2][kMaxTop + 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int C = (int)cluster_size(), rank = (int)cluster_rank(), clusters = gridDim.x / C, first = rank * per;
   if (tid == 0) {
@@ -396,6 +434,8 @@ __global__ void __launch_bounds__(kThreads, 1280 / kThreads)
   const Weights w = call_weights<kThreads>(rows, call, red);
   const float d = dloss ? *dloss : 1.f;
   const float w_taught = (float)(w.taught * (double)call.temperature) * d, w_labelled = (float)w.labelled * d;
+  const double loss_taught = w.taught * (double)call.temperature * (double)call.temperature * kLn2;
+  const double loss_labelled = w.labelled * kLn2;
   const int taken = cnt ? *cnt : places;
   // rows behind the last taken one are not read again, except that the weight gradient's last block of 64 rows (the first
   // one if there is none) has to end in zeros
@@ -423,6 +463,18 @@ __global__ void __launch_bounds__(kThreads, 1280 / kThreads)
   int place = blockIdx.x / C, next = place + clusters;
   int at = place < end ? row_at(place) : -1, mark = mark_of(at);
   if (tid == 0 && mark != 0) fetch(place);
+  const int K1 = rows.K + 1;
+  // A row's slots on their way into shared memory.
+  auto fetch_slots = [&](int at, int turn) {
+    for (int j = tid; j < K1; j += kThreads) {
+      const long q = (long)at * K1 + j;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&slot_ids[turn][j])), "l"(rows.slot_id + q)
+                   : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&slot_ps[turn][j])), "l"(rows.slot_p + q)
+                   : "memory");
+    }
+  };
+  if (mark != 0) fetch_slots(at, 0);
   uint32_t phase = 0;
   for (int k = 0; place < end; ++k) {
     const int turn = k & 1;
@@ -435,29 +487,16 @@ __global__ void __launch_bounds__(kThreads, 1280 / kThreads)
     const int o_lead = Row<T>::lead_for(o);
     const int next_at = next < end ? row_at(next) : -1, next_mark = mark_of(next_at);
     if (mark != 0) {
-      if (tid == 32 && next_mark != 0) {
-        const Row<T> ahead = row_of(next);
-        const int2 r = whole(ahead, max(min(per, ahead.vectors() - first), 0));
-        if (r.x < r.y)
-          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(ahead.p + ahead.column(first + r.x)),
-                       "r"((r.y - r.x) * 16)
-                       : "memory");
-      }
       if (tid >= 64 && tid < 64 + n - (mid.y - mid.x)) {
         const int i = tid == 64 && mid.x ? 0 : n - 1;
         held[i] = row.load(first + i);
-      }
-      for (int j = tid; j <= rows.K; j += kThreads) {
-        const long q = (long)at * (rows.K + 1) + j;
-        const int id = rows.slot_id[q];
-        slots[turn][j] = make_float2(id >= 0 ? rows.slot_p[q] : 0.f, id >= 0 ? to_float(row.p[id]) : 0.f);
-        slot_ids[turn][j] = id;
       }
       // one warp waits for the copy, the others without issuing anything at the barrier
       if (mid.x < mid.y) {
         if (warp == 0) mbar_wait(&arrived, phase, ew, 710);
         phase ^= 1;
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
       __syncthreads();
       float m = -INFINITY;
 #pragma unroll 4
@@ -465,19 +504,23 @@ __global__ void __launch_bounds__(kThreads, 1280 / kThreads)
       m = warp_top(m);
       // a warp that has nothing but -inf adds zeros (2^-inf), not 2^(-inf + inf)
       const float t = m == -INFINITY ? 0.f : __fmul_rn(m, call.c), t1 = m == -INFINITY ? 0.f : __fmul_rn(m, call.c1);
-      float s = 0.f, s1 = 0.f;
+      f32x2 s2 = both(0.f, 0.f), s12 = s2;
+      {
+        const Powers pw(call, t, t1, squares);
 #pragma unroll 2
-      for (int i = tid; i < n; i += kThreads) {
-        float v[kVec];
-        RowVec<T>::unpack(held[i], v);
+        for (int i = tid; i < n; i += kThreads) {
+          float v[kVec];
+          RowVec<T>::unpack(held[i], v);
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          const float2 e = powers<kMode>(v[j], call, t, t1, squares);
-          s += e.x;
-          if constexpr (kDual) s1 += e.y;
+          for (int j = 0; j < kVec; j += 2) {
+            f32x2 e, e1;
+            pw.take<kMode>(both(v[j], v[j + 1]), e, e1);
+            s2 = add2(s2, e);
+            if constexpr (kDual) s12 = add2(s12, e1);
+          }
         }
       }
-      s = warp_sum(s);
+      float s = warp_sum(apart(s2).x + apart(s2).y), s1 = apart(s12).x + apart(s12).y;
       if constexpr (kDual) s1 = warp_sum(s1);
       if (lane == 0) warp_part[warp] = make_float4(m, s, s1, 0.f);
       __syncthreads();
@@ -522,9 +565,21 @@ __global__ void __launch_bounds__(kThreads, 1280 / kThreads)
       const int label_at = mark & kLabelled ? mark >> kSlotShift : -1;
       const float wt = mark & kTaught ? w_taught : 0.f, wl = mark & kLabelled ? w_labelled : 0.f;
       const float a = (kDual ? wt : wt + wl) / S, a1 = kDual ? wl / S1 : 0.f;
-      auto grad = [&](float x) {
-        const float2 e = powers<kMode>(x, call, t, t1, squares);
-        return kDual ? __fmaf_rn(a, e.x, a1 * e.y) : a * e.x;
+      const Powers pw(call, t, t1, squares);
+      const f32x2 a2 = both(a, a), a12 = both(a1, a1);
+      auto grad = [&](float x, float y) {
+        f32x2 e, e1;
+        pw.take<kMode>(both(x, y), e, e1);
+        return apart(kDual ? fma2(a2, e, mul2(a12, e1)) : mul2(a2, e));
+      };
+      auto grads = [&](int i, float (&v)[kVec]) {
+        RowVec<T>::unpack(held[i], v);
+#pragma unroll
+        for (int j = 0; j < kVec; j += 2) {
+          const float2 g = grad(v[j], v[j + 1]);
+          v[j] = g.x;
+          v[j + 1] = g.y;
+        }
       };
       if (o) {
         const bool in_step = o_lead == row.lead;   // whole vectors may be stored whole
@@ -532,50 +587,64 @@ __global__ void __launch_bounds__(kThreads, 1280 / kThreads)
 #pragma unroll 2
         for (int i = lo + tid; i < hi; i += kThreads) {
           float v[kVec];
-          RowVec<T>::unpack(held[i], v);
-#pragma unroll
-          for (int j = 0; j < kVec; ++j) v[j] = grad(v[j]);
+          grads(i, v);
           if (in_step) Row<T>::store_whole(o + row.column(first + i), v);
           else row.store(o, o_lead, first + i, v);
         }
         if (tid >= kThreads - n + (hi - lo)) {     // the others
           const int i = tid == kThreads - 1 && lo ? 0 : n - 1;
           float v[kVec];
-          RowVec<T>::unpack(held[i], v);
-#pragma unroll
-          for (int j = 0; j < kVec; ++j) v[j] = grad(v[j]);
+          grads(i, v);
           row.store(o, o_lead, first + i, v);
         }
       }
-      __syncthreads();                             // `held` may be written again; a slot's logit was another thread's
-      if (tid == 0 && next_mark != 0) fetch(next);
-      if (o)
-        for (int j = tid; j <= rows.K; j += kThreads) {
-          const int id = slot_ids[turn][j];
-          if (id < 0 || (unsigned)((id + row.lead) / kVec - first) >= (unsigned)n) continue;
-          float g = grad(slots[turn][j].y) - wt * slots[turn][j].x;
-          if (j == label_at) g -= wl;
-          from_float(g, o + id);
-        }
-      if (warp == kWarps - 1 && place % C == rank) {
-        double dot = 0.0;
-        for (int j = lane; j <= rows.K; j += 32)
-          if (!(slots[turn][j].x == 0.f)) dot += (double)slots[turn][j].x * (double)slots[turn][j].y;
+      // the slots that this CTA holds: their gradients (two slots a thread at most), and one warp's part of the row's loss
+      auto held_slot = [&](int j, int& id, float& p, float& x) {
+        id = j < K1 ? slot_ids[turn][j] : -1;
+        if (id < 0 || (unsigned)((id + row.lead) / kVec - first) >= (unsigned)n) return false;
+        p = slot_ps[turn][j];
+        x = to_float(reinterpret_cast<const T*>(held)[id + row.lead - first * kVec]);
+        return true;
+      };
+      int id;
+      float p, x, fix[2];
+      int fix_at[2] = {-1, -1};
 #pragma unroll
-        for (int q = 16; q > 0; q >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, q);
+      for (int b = 0; b < 2; ++b) {
+        const int j = tid + b * kThreads;
+        if (!held_slot(j, id, p, x)) continue;
+        fix_at[b] = id;
+        fix[b] = grad(x, x).x - wt * p - (j == label_at ? wl : 0.f);
+      }
+      double part_loss = 0.0;
+      if (warp == kWarps - 1) {
+        const double lse = (double)t + log2((double)S), lse1 = kDual ? (double)t1 + log2((double)S1) : lse;
+        for (int j = lane; j < K1; j += 32)
+          if (held_slot(j, id, p, x)) {
+            if (!(p == 0.f)) part_loss += loss_taught * (double)p * (lse - (double)x * (double)call.c);
+            if (j == label_at) part_loss += loss_labelled * (lse1 - (double)x * (double)call.c1);
+          }
+      }
+      __syncthreads();                             // `held` may be written again; a slot's gradient was another thread's
+      if (tid == 0 && next_mark != 0) fetch(next);
+      if (o) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          if (fix_at[b] >= 0) from_float(fix[b], o + fix_at[b]);
+      }
+      if (warp == kWarps - 1) {
+#pragma unroll
+        for (int q = 16; q > 0; q >>= 1) part_loss += __shfl_xor_sync(0xffffffffu, part_loss, q);
         if (lane == 0) {
-          stats[kTop * n_rows + at] = t;
-          stats[kTop1 * n_rows + at] = t1;
-          stats[kSum * n_rows + at] = S;
-          stats[kSum1 * n_rows + at] = kDual ? S1 : S;
-          stats[kDot * n_rows + at] = dot;
-          stats[kLabel * n_rows + at] = label_at >= 0 ? (double)slots[turn][label_at].y : 0.0;
+          if (rank == 0 && (mark & kTaught) && loss_taught > 0.0) part_loss += loss_taught / kLn2 * rows.info[at].x;
+          stats[(long)rank * n_rows + at] = part_loss;
         }
       }
     } else {
       __syncthreads();                             // all have read the ticket
       if (tid == 0 && next_mark != 0) fetch(next);
     }
+    if (next_mark != 0) fetch_slots(next_at, turn ^ 1);
     place = next;
     next = after;
     at = next_at;
@@ -586,30 +655,50 @@ __global__ void __launch_bounds__(kThreads, 1280 / kThreads)
 }
 
 // ----------------------------------------------------------------------------
-// The loss of all rows, in the order of the rows: one CTA.
+// Losses of the rows from their statistics, into the place of the first of them.
 // ----------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) distill_row_loss_kernel(DistillRows rows, DistillCall call, long n_rows,
+                                                               double* stats) {
+  grid_dependency_sync();
+  __shared__ int red[8];
+  const Weights w = call_weights<256>(rows, call, red);
+  const long r = blockIdx.x * 256L + threadIdx.x;
+  if (r >= n_rows) return;
+  const int mark = rows.mark[r];
+  double loss = 0.0;
+  if ((mark & kTaught) && w.taught > 0.0) {
+    const double2 info = rows.info[r];
+    const double lse = stats[kTop * n_rows + r] + log2(stats[kSum * n_rows + r]);
+    const double kl = info.x - kLn2 * (stats[kDot * n_rows + r] * (double)call.c - info.y * lse);
+    loss += w.taught * (double)call.temperature * (double)call.temperature * kl;
+  }
+  if ((mark & kLabelled) && w.labelled > 0.0) {
+    const double lse = stats[kTop1 * n_rows + r] + log2(stats[kSum1 * n_rows + r]);
+    loss += w.labelled * kLn2 * (lse - stats[kLabel * n_rows + r] * (double)call.c1);
+  }
+  stats[r] = loss;
+}
+
+// The sum of n losses, always in the same order: one CTA.
 constexpr int kLossThreads = 1024;
-__global__ void __launch_bounds__(kLossThreads) distill_loss_kernel(DistillRows rows, DistillCall call, long n_rows,
-                                                                   const double* stats, float* __restrict__ loss) {
+__global__ void __launch_bounds__(kLossThreads) distill_loss_kernel(const double* losses, long n, float* __restrict__ loss) {
   grid_dependency_sync();
   __shared__ double dred[kLossThreads / 32];
-  __shared__ int red[kLossThreads / 32];
-  const Weights w = call_weights<kLossThreads>(rows, call, red);
-  double total = 0.0;
-  for (long r = threadIdx.x; r < n_rows; r += kLossThreads) {
-    const int mark = rows.mark[r];
-    if ((mark & kTaught) && w.taught > 0.0) {
-      const double2 info = rows.info[r];
-      const double lse = stats[kTop * n_rows + r] + log2(stats[kSum * n_rows + r]);
-      const double kl = info.x - kLn2 * (stats[kDot * n_rows + r] * (double)call.c - info.y * lse);
-      total += w.taught * (double)call.temperature * (double)call.temperature * kl;
-    }
-    if ((mark & kLabelled) && w.labelled > 0.0) {
-      const double lse = stats[kTop1 * n_rows + r] + log2(stats[kSum1 * n_rows + r]);
-      total += w.labelled * kLn2 * (lse - stats[kLabel * n_rows + r] * (double)call.c1);
-    }
-  }
-  total = block_total<kLossThreads>(total, dred);
+  double part[4] = {0.0, 0.0, 0.0, 0.0};
+  long i = threadIdx.x;
+  for (; i + 3 * kLossThreads < n; i += 4 * kLossThreads)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) part[q] += losses[i + q * kLossThreads];
+  for (; i < n; i += kLossThreads) part[0] += losses[i];
+  double total = (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if ((threadIdx.x & 31) == 0) dred[threadIdx.x >> 5] = total;
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  total = dred[threadIdx.x];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (threadIdx.x == 0) *loss = (float)total;
 }
 
@@ -653,6 +742,7 @@ struct MmtDistill {
   const float* dloss;
   double temperature, share;
   int V, K, is_f32, out_f32;
+  int parts;                        // of a row's loss in `stats`, 0: its statistics; set by the kernels' calls
 };
 
 namespace {
@@ -693,7 +783,8 @@ long row_vectors(const MmtDistill& d) {
 constexpr int kHeldBytes = 40 * 1024, kMaxHeldBytes = 200 * 1024;
 
 template <typename T, typename O, int kThreads, int kMode>
-int launch_held(const MmtDistill& d, int C, int per, int squares, void* stream) {
+int launch_held(MmtDistill& d, int C, int per, int squares, void* stream) {
+  d.parts = C;
   auto kernel = distill_fused_kernel<T, O, kThreads, kMode>;
   static int allowed = 0;
   const int bytes = per * 16;
@@ -715,7 +806,7 @@ int launch_held(const MmtDistill& d, int C, int per, int squares, void* stream) 
                              per, mmt_error_word());
 }
 template <typename T, typename O, int kMode>
-int launch_mode(const MmtDistill& d, int squares, void* stream) {
+int launch_mode(MmtDistill& d, int squares, void* stream) {
   const long nv = row_vectors(d);
   // as few CTAs a row as hold it in 40 KB each, of which five fit an SM; more where there are few rows
   int C = 1;
@@ -726,7 +817,7 @@ int launch_mode(const MmtDistill& d, int squares, void* stream) {
                                 : launch_held<T, O, 512, kMode>(d, C, per, squares, stream);
 }
 template <typename T, typename O>
-int launch_fused(const MmtDistill& d, void* stream) {
+int launch_fused(MmtDistill& d, void* stream) {
   if (!dual(d)) return launch_mode<T, O, kSingle>(d, 0, stream);
   if (d.temperature == 2.0 || d.temperature == 4.0 || d.temperature == 8.0)
     return launch_mode<T, O, kSquares>(d, d.temperature == 2.0 ? 1 : d.temperature == 4.0 ? 2 : 3, stream);
@@ -739,6 +830,8 @@ extern "C" {
 
 // Size of MmtDistill, for the caller to agree on.
 int mmt_distill_bytes() { return (int)sizeof(MmtDistill); }
+// Values that `stats` has per row.
+int mmt_distill_stats_count() { return kStats; }
 // Rows that share one entry of `counts`.
 int mmt_distill_count_rows() { return kPrepareRows; }
 
@@ -753,14 +846,15 @@ int mmt_distill_prepare(const MmtDistill* d, const long* ids, long ids_ld, const
   if (teacher_f32)
     return (int)launch_dependent(distill_prepare_kernel<float>, grid, 32 * kPrepareRows, 0, VR_STREAM(stream), ids, ids_ld,
                                  reinterpret_cast<const float*>(teacher), teacher_ld, labels, d->rows, vocab, inv,
-                                 rows_of(*d), need, d->ticket, mmt_error_word());
+                                 rows_of(*d), need, d->stats, d->ticket, mmt_error_word());
   return (int)launch_dependent(distill_prepare_kernel<bf16>, grid, 32 * kPrepareRows, 0, VR_STREAM(stream), ids, ids_ld,
                                reinterpret_cast<const bf16*>(teacher), teacher_ld, labels, d->rows, vocab, inv, rows_of(*d),
-                               need, d->ticket, mmt_error_word());
+                               need, d->stats, d->ticket, mmt_error_word());
 }
 
-int mmt_distill_stats(const MmtDistill* d, void* stream) {
+int mmt_distill_stats(MmtDistill* d, void* stream) {
   if (wrong(*d)) return -2;
+  d->parts = 0;
   if (d->places == 0) return 0;
   if (d->is_f32) return dual(*d) ? launch_stats<float, true>(*d, stream) : launch_stats<float, false>(*d, stream);
   return dual(*d) ? launch_stats<bf16, true>(*d, stream) : launch_stats<bf16, false>(*d, stream);
@@ -780,23 +874,29 @@ long mmt_distill_fused_columns(int is_f32) {
 }
 
 // Statistics of a whole vocabulary and, unless `out` is null, the gradient (times *dloss, if that is not null).
-int mmt_distill_fused(const MmtDistill* d, void* stream) {
+int mmt_distill_fused(MmtDistill* d, void* stream) {
   if (wrong(*d) || (d->out_f32 && !d->is_f32) || d->V > mmt_distill_fused_columns(d->is_f32)) return -2;
   if (d->places == 0) return 0;
   if (d->out_f32) return launch_fused<float, float>(*d, stream);
   return d->is_f32 ? launch_fused<float, bf16>(*d, stream) : launch_fused<bf16, bf16>(*d, stream);
 }
 
+// From the statistics (parts == 0) or from the losses that mmt_distill_fused has left: `parts` for each row.
 int mmt_distill_loss(const MmtDistill* d, float* loss, void* stream) {
-  if (wrong(*d)) return -2;
-  return (int)launch_dependent(distill_loss_kernel, 1, kLossThreads, 0, VR_STREAM(stream), rows_of(*d), call_of(*d), d->rows,
-                               d->stats, loss);
+  if (wrong(*d) || d->parts < 0 || d->parts > kMaxCluster) return -2;
+  if (d->parts == 0 && d->rows > 0) {
+    const int e = (int)launch_dependent(distill_row_loss_kernel, (unsigned)((d->rows + 255) / 256), 256, 0, VR_STREAM(stream),
+                                        rows_of(*d), call_of(*d), d->rows, d->stats);
+    if (e) return e;
+  }
+  return (int)launch_dependent(distill_loss_kernel, 1, kLossThreads, 0, VR_STREAM(stream), d->stats,
+                               d->rows * (d->parts ? d->parts : 1), loss);
 }
 
 // n values at a 16-byte boundary.
 int mmt_distill_scale(void* grad, int is_f32, long n, const float* factor, void* stream) {
   if (n == 0) return 0;
-  const long vecs = (n + 7) / 8, want = (vecs + 255) / 256, most = 8L * mmt_sm_count();
+  const long vecs = (n + 7) / 8, want = (vecs + 255) / 256, most = 4L * mmt_sm_count();
   const unsigned grid = (unsigned)(want < most ? want : most);
   return is_f32 ? (int)launch_dependent(distill_scale_kernel<float>, grid, 256, 0, VR_STREAM(stream),
                                         reinterpret_cast<float*>(grad), n, factor)

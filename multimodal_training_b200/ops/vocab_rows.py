@@ -149,11 +149,12 @@ class _DistillWords(ctypes.Structure):
                 ("info", ctypes.c_void_p), ("mark", ctypes.c_void_p), ("counts", ctypes.c_void_p),
                 ("stats", ctypes.c_void_p), ("ticket", ctypes.c_void_p), ("dloss", ctypes.c_void_p),
                 ("temperature", ctypes.c_double), ("share", ctypes.c_double), ("V", ctypes.c_int), ("K", ctypes.c_int), ("is_f32", ctypes.c_int),
-                ("out_f32", ctypes.c_int)]
+                ("out_f32", ctypes.c_int), ("parts", ctypes.c_int)]
 
 
 nv.declare("mmt_distill_bytes", nv.c_int, [])
 nv.declare("mmt_distill_count_rows", nv.c_int, [])
+nv.declare("mmt_distill_stats_count", nv.c_int, [])
 nv.declare("mmt_distill_prepare", nv.c_int, [nv._P, nv._P, nv.c_long, nv._P, nv.c_long, nv.c_int, nv._P, nv.c_long, nv._P,
                                              nv._P])
 nv.declare("mmt_distill_stats", nv.c_int, [nv._P, nv._P])
@@ -173,9 +174,8 @@ class _Distill:
         rows, K = teacher_ids.shape
         dev = teacher_ids.device
         per = nv.lib().mmt_distill_count_rows()
-        # one buffer: info [rows, 2] and stats [6, rows] in fp64, then slots of 4 bytes
         n_counts = (rows + per - 1) // per
-        self.stats = torch.empty(6, rows, device=dev, dtype=torch.float64)
+        self.stats = torch.empty(nv.lib().mmt_distill_stats_count(), rows, device=dev, dtype=torch.float64)
         self.info = torch.empty(rows, 2, device=dev, dtype=torch.float64)
         self.small = torch.empty(2 * rows * (K + 1) + rows + 2 * n_counts + 2, device=dev, dtype=torch.int32)
         at = self.small.data_ptr()
@@ -210,12 +210,12 @@ class _Distill:
         top = self.stats[:2, lo:hi].contiguous()
         mine = top.clone()
         F._all_reduce(top, torch.distributed.ReduceOp.MAX, group)
-        rest = self.stats[2:, lo:hi].contiguous()
+        rest = self.stats[2:6, lo:hi].contiguous()
         # a shard of nothing but -inf has a sum of zero, which stays
         rest[:2] = torch.where(rest[:2] > 0, rest[:2] * torch.exp2(mine - top), rest[:2])
         F._all_reduce(rest, torch.distributed.ReduceOp.SUM, group)
         self.stats[:2, lo:hi] = top
-        self.stats[2:, lo:hi] = rest
+        self.stats[2:6, lo:hi] = rest
 
     def _out(self, out, dloss=None) -> None:
         w = self.words
