@@ -409,7 +409,7 @@ struct Powers {
 };
 
 template <typename T, typename O, int kThreads, int kMode>
-__global__ void __launch_bounds__(kThreads, 1280 / kThreads)
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     distill_fused_kernel(const T* logits, long ld, int V, DistillRows rows, DistillCall call, int squares, long n_rows,
                          int places, const long* src, const int* cnt, double* __restrict__ stats, int* ticket,
                          const float* dloss, O* out, long out_ld, int per, MmtErrorWord* ew) {
@@ -808,7 +808,7 @@ int launch_held(MmtDistill& d, int C, int per, int squares, void* stream) {
 template <typename T, typename O, int kMode>
 int launch_mode(MmtDistill& d, int squares, void* stream) {
   const long nv = row_vectors(d);
-  // as few CTAs a row as hold it in 40 KB each, of which five fit an SM; more where there are few rows
+  // as few CTAs a row as hold it in 40 KB each, of which an SM has four; more where there are few rows
   int C = 1;
   while (C < kMaxCluster && nv * 16 > (long)kHeldBytes * C) C *= 2;
   while (C < kMaxCluster && d.places * C * 2 <= 2 * mmt_sm_count() && nv > 512L * C) C *= 2;

@@ -155,6 +155,15 @@ MMT_DEVICE void cluster_send(float4* p, uint64_t* bar, uint32_t rank, float4 v) 
                : "memory");
 }
 
+// Reads the place in CTA `rank`'s shared memory that `p` has in this CTA's.
+MMT_DEVICE unsigned long long cluster_load(const unsigned long long* p, uint32_t rank) {
+  uint32_t a;
+  unsigned long long v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+  return v;
+}
+
 // mbar_wait (common.cuh) for what other CTAs of the cluster have sent.
 MMT_DEVICE bool cluster_wait(uint64_t* bar, uint32_t parity, MmtErrorWord* ew, int where) {
   const uint32_t addr = smem_u32(bar);
