@@ -4,11 +4,12 @@
 // torch.topk has it; -0 equal to +0) above the inverted column, so that keys are unique and equal logits go by the lower
 // column.  The answer is the k largest keys of the row.
 //
-// One pass over the row, bound by memory: what is left of each stretch of logits is what reaches a lower bound of the k-th
-// largest logit.  The bound is the k-th largest of the threads' own largest logits, which are k different elements; a row in
-// no special order leaves about k (1 + 1 + 1/2 + ...) candidates.  They are ranked by counting.  Rows in rising order, or
-// with many equal logits, overflow the list of candidates; such a row is selected digit by digit from histograms instead,
-// with further passes over it.
+// One pass over the row, bound by memory: what is left of the logits is what reaches a lower bound of the k-th largest.  The
+// bound is the k-th largest of the threads' own largest logits so far, which are k different elements; it is raised behind
+// stretches 1, 2, 4, ... of the row, and a row in no special order leaves about k (1 + 1 + 1/2 + ...) candidates.  Where the
+// list of candidates fills up all the same (rising logits, many equal ones) it is cut to the k largest, of which the last is
+// the next bound; columns only grow, so equal logits that come later do not reach it.  In the end the candidates are cut to
+// those near the k-th largest by histograms and ranked by counting.
 //
 // Few rows are cut into runs of columns, one for each CTA of a cluster; the first CTA ranks the others' lists.
 #include "vocab_rows.cuh"
@@ -17,12 +18,11 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kTopThreads = 512;
-constexpr int kTopWarps = kTopThreads / 32;
 constexpr int kTopMax = 256;          // largest k
-constexpr int kTopList = 2048;        // candidates that are kept
-constexpr int kTopAhead = 4;          // vectors that a thread loads before it looks at them
+constexpr int kTopSets = 4;           // vectors that a thread loads ahead: one of each set
+constexpr int kTopFull = 1024;        // candidates from which on the list is cut
 constexpr int kTopCluster = 8;        // most CTAs of a row; their lists fit one list: 8 * 256 = 2048
+constexpr int kTopBins = 256;
 
 // Order-preserving bits of a logit; kBits of them.
 template <typename T>
@@ -50,7 +50,7 @@ struct Key<float> {
   static constexpr int kBits = 32;
   static MMT_DEVICE uint32_t of(float x) {
     uint32_t b = __float_as_uint(x);
-    if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+    if ((b & 0x7fffffffu) > 0x7f800000u) return 0xfffffffeu;          // one below the largest: there is a key above it
     if (b == 0x80000000u) b = 0;
     return b & 0x80000000u ? ~b : b | 0x80000000u;
   }
@@ -63,6 +63,19 @@ struct Key<float> {
   }
 };
 
+// Element j (of as many as a vector has) of a vector.
+template <typename T>
+MMT_DEVICE T element(const uint4& v, int j);
+template <>
+MMT_DEVICE bf16 element<bf16>(const uint4& v, int j) {
+  const uint32_t w = j & 4 ? (j & 2 ? v.w : v.z) : (j & 2 ? v.y : v.x);
+  return __ushort_as_bfloat16((unsigned short)(j & 1 ? w >> 16 : w));
+}
+template <>
+MMT_DEVICE float element<float>(const uint4& v, int j) {
+  return __uint_as_float(j & 2 ? (j & 1 ? v.w : v.z) : (j & 1 ? v.y : v.x));
+}
+
 // A CTA's run of a row: vectors [first, stop).
 template <typename T>
 struct Run {
@@ -70,147 +83,111 @@ struct Run {
   int first, stop;
 };
 
+template <int kTopThreads>
 struct TopShared {
-  u64 list[kTopList];
+  u64 list[kTopFull + 8 * kTopThreads];          // all elements of a set fit behind a list that is not full
   u64 best[kTopMax];
-  int hist[256];
-  int found[3];
+  int hist[kTopBins];
+  int digit, need, count;               // of find_digit
   int taken, kept;
-  int warp_count[kTopWarps];
+  uint32_t warp_value[2][32];
 };
 
-// Calls f(key, column) for every element of vector i that the row has.
-template <typename T, typename F>
-MMT_DEVICE void each_key(const Row<T>& row, int i, const uint4& u, F f) {
-  const T* e = reinterpret_cast<const T*>(&u);
-  const int c = row.column(i);
-#pragma unroll
-  for (int j = 0; j < Row<T>::kVec; ++j)
-    if (c + j >= 0 && c + j < row.V) f(Key<T>::of(e[j]), c + j);
-}
-template <typename T, typename F>
-MMT_DEVICE void each_key(const Row<T>& row, int i, F f) {
-  each_key<T>(row, i, row.load(i), f);
-}
 MMT_DEVICE u64 whole_key(uint32_t key, int c) { return (u64)key << 32 | (0xffffffffu - (uint32_t)c); }
 
-// The largest t of 16 bits that at least k of the block's values reach (0 if there are fewer than k).  A thread has N
-// values, of which the first `n` (the same for all threads) count.
-template <int N>
-MMT_DEVICE uint32_t kth_of_block(const uint32_t (&v)[N], int n, int k) {
-  uint32_t t = 0;
-  for (int bit = 15; bit >= 0; --bit) {
-    const uint32_t at = t | 1u << bit;
-    int count = 0;
+// Sum over the lanes up to this one.
+MMT_DEVICE int up_to_lane(int v) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (j < n) count += __syncthreads_count(v[j] >= at);
-    if (count >= k) t = at;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int w = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += w;
   }
-  return t;
+  return v;
 }
-
-// best[0, k) := the k largest keys of a run that has at least k elements, in no order.  Digits of 8 bits from histograms.
-template <typename T>
-MMT_DEVICE void select_by_digits(const Run<T>& run, int k, TopShared& s) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const Row<T>& row = run.row;
-  uint32_t prefix = 0, mask = 0;
-  int need = k;
-  for (int shift = Key<T>::kBits - 8; shift >= 0; shift -= 8) {
-    __syncthreads();
-    for (int b = tid; b < 256; b += kTopThreads) s.hist[b] = 0;
-    __syncthreads();
-    for (int i = run.first + tid; i < run.stop; i += kTopThreads)
-      each_key<T>(row, i, [&](uint32_t key, int) {
-        if ((key & mask) == prefix) atomicAdd(&s.hist[key >> shift & 255u], 1);
-      });
-    __syncthreads();
-    if (warp == 0) {
-      // lane l holds the eight digits from 255 - 8 l down
-      int mine = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) mine += s.hist[255 - 8 * lane - j];
-      int before = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += v;
-      }
-      before -= mine;                            // keys above this lane's digits
-      if (before < need && before + mine >= need) {
-        int d = 255 - 8 * lane;
-        while (before + s.hist[d] < need) before += s.hist[d--];
-        s.found[0] = d;
-        s.found[1] = need - before;
-        s.found[2] = s.hist[d];
-      }
-    }
-    if (tid == 0) s.taken = 0;
-    __syncthreads();
-    prefix |= (uint32_t)s.found[0] << shift;
-    mask |= 255u << shift;
-    need = s.found[1];
-  }
-  const bool all_ties = s.found[2] == need;
-  for (int i = run.first + tid; i < run.stop; i += kTopThreads)
-    each_key<T>(row, i, [&](uint32_t key, int c) {
-      if (key > prefix || (all_ties && key == prefix)) s.best[atomicAdd(&s.taken, 1)] = whole_key(key, c);
-    });
+// Smallest and largest of a block's values.
+template <int kTopThreads>
+MMT_DEVICE uint2 range_of_block(TopShared<kTopThreads>& s, uint32_t v) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t lo = __reduce_min_sync(0xffffffffu, v), hi = __reduce_max_sync(0xffffffffu, v);
   __syncthreads();
-  if (all_ties) return;
-  // the lowest columns among equals: whole blocks of vectors in the order of the columns
-  int place = s.taken;
-  for (int i0 = run.first; i0 < run.stop && place < k; i0 += kTopThreads) {
-    int mine = 0;
-    if (i0 + tid < run.stop) each_key<T>(row, i0 + tid, [&](uint32_t key, int) { mine += key == prefix; });
-    int before = mine;
+  if (lane == 0) {
+    s.warp_value[0][warp] = lo;
+    s.warp_value[1][warp] = hi;
+  }
+  __syncthreads();
+  return make_uint2(__reduce_min_sync(0xffffffffu, s.warp_value[0][lane % (kTopThreads / 32)]),
+                    __reduce_max_sync(0xffffffffu, s.warp_value[1][lane % (kTopThreads / 32)]));
+}
+// The largest t that at least k of the block's values reach; k is at most the block's size.
+template <int kTopThreads>
+MMT_DEVICE uint32_t kth_of_block(TopShared<kTopThreads>& s, uint32_t v, int k) {
+  uint2 r = range_of_block<kTopThreads>(s, v);
+  while (r.x < r.y) {
+    const uint32_t at = (r.x + r.y + 1) / 2;
+    if (__syncthreads_count(v >= at) >= k) r.x = at;
+    else r.y = at - 1;
+  }
+  return r.x;
+}
+// The bin at which the counts, from the last bin down, reach `need`, how many of it are needed and how many there are, into
+// shared memory.  All of the block calls it; the barrier behind it is the caller's.
+template <int kTopThreads>
+MMT_DEVICE void find_digit(TopShared<kTopThreads>& s, int need) {
+  if (threadIdx.x >= 32) return;
+  constexpr int kEach = kTopBins / 32;
+  // lane l holds the bins from kTopBins - 1 - kEach * l down
+  const int from = kTopBins - 1 - kEach * (int)threadIdx.x;
+  int mine = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane >= o) before += v;
-    }
-    if (lane == 31) s.warp_count[warp] = before;
-    before -= mine;
-    __syncthreads();
-    int total = 0;
-#pragma unroll
-    for (int w = 0; w < kTopWarps; ++w) {
-      before += w < warp ? s.warp_count[w] : 0;
-      total += s.warp_count[w];
-    }
-    int at = place + before;
-    if (mine && at < k)
-      each_key<T>(row, i0 + tid, [&](uint32_t key, int c) {
-        if (key == prefix && at < k) s.best[at++] = whole_key(key, c);
-      });
-    place += total;
-    __syncthreads();
+  for (int j = 0; j < kEach; ++j) mine += s.hist[from - j];
+  int before = up_to_lane(mine) - mine;          // keys above this lane's bins
+  if (before < need && before + mine >= need) {
+    int d = from;
+    while (before + s.hist[d] < need) before += s.hist[d--];
+    s.digit = d;
+    s.need = need - before;
+    s.count = s.hist[d];
   }
 }
 
-// Ranks the n keys of the list that reach `bound` (16 bits of a logit's order) and hands out the k largest: out(rank, key).
-// At least k do.  `shift`: of the 16 bits in a key.
-template <typename F>
-MMT_DEVICE void rank_list(TopShared& s, int n, int k, int shift, F out) {
+// Ranks the n keys of the list and hands out the k largest: out(rank, key).  n >= k, and k of the keys reach `bound` (16 bits
+// from `shift` up).  All threads come out of it together.
+template <int kTopThreads, typename F>
+MMT_DEVICE void rank_list(TopShared<kTopThreads>& s, int n, int k, int shift, uint32_t bound, F out) {
   const int tid = threadIdx.x;
-  constexpr int kEach = kTopList / kTopThreads;
-  u64 mine[kEach];
-  uint32_t v[kEach];
-#pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    const int i = tid + j * kTopThreads;
-    mine[j] = i < n ? s.list[i] : 0;
-    v[j] = (uint32_t)(mine[j] >> shift) & 0xffffu;
-  }
-  if (n > 64) {                                     // what cannot be among the k leaves the list
-    const uint32_t t = kth_of_block(v, (n + kTopThreads - 1) / kTopThreads, k);
-    if (tid == 0) s.kept = 0;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kEach; ++j)
-      if (mine[j] != 0 && v[j] >= t) s.list[atomicAdd(&s.kept, 1)] = mine[j];
-    __syncthreads();
+  if (n > 64 && n > k) {                          // what cannot be among the k leaves the list
+    uint32_t most = 0;
+    for (int i = tid; i < n; i += kTopThreads) most = max(most, (uint32_t)(s.list[i] >> shift) & 0xffffu);
+    most = range_of_block<kTopThreads>(s, most).y;
+    // keys in [low, low + bins) compete for `need` places; those above have theirs
+    u64 low = (u64)bound << shift;
+    int wide = shift + 32 - __clz((most - bound) / kTopBins), need = k, sure = 0;
+    for (;;) {
+      for (int b = tid; b < kTopBins; b += kTopThreads) s.hist[b] = 0;
+      if (tid == 0) s.kept = 0;
+      __syncthreads();
+      for (int i = tid; i < n; i += kTopThreads) {
+        const u64 key = s.list[i];
+        if (key >= low && (key - low) >> wide < kTopBins) atomicAdd(&s.hist[(int)((key - low) >> wide)], 1);
+      }
+      __syncthreads();
+      find_digit(s, need);
+      __syncthreads();
+      low += (u64)s.digit << wide;
+      sure += need - s.need;
+      need = s.need;
+      const int left = sure + s.count;
+      if (left <= k + 128 || wide == 0) break;
+      wide = max(wide - 8, 0);
+      __syncthreads();                            // all have read what find_digit found
+    }
+    for (int i0 = 0; i0 < n; i0 += kTopThreads) { // in place: what is written has been read
+      const u64 key = i0 + tid < n ? s.list[i0 + tid] : 0;
+      __syncthreads();
+      if (key != 0 && key >= low) s.list[atomicAdd(&s.kept, 1)] = key;
+      __syncthreads();
+    }
     n = s.kept;
   }
   for (int i = tid; i < n; i += kTopThreads) {
@@ -219,15 +196,17 @@ MMT_DEVICE void rank_list(TopShared& s, int n, int k, int shift, F out) {
     for (int j = 0; j < n; ++j) rank += s.list[j] > key;
     if (rank < k) out(rank, key);
   }
+  __syncthreads();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kTopThreads, 3) top_logits_kernel(const T* logits, T* __restrict__ values,
-                                                                    long* __restrict__ ids, int V, long ld, int k,
-                                                                    long vocab_lo, int per) {
+template <typename T, int kTopThreads>
+__global__ void __launch_bounds__(kTopThreads, 1024 / kTopThreads) top_logits_kernel(const T* logits, T* __restrict__ values,
+                                                                                    long* __restrict__ ids, int V, long ld,
+                                                                                    int k, long vocab_lo, int per) {
   grid_dependency_sync();
-  __shared__ TopShared s;
-  const int tid = threadIdx.x;
+  constexpr int kStretch = kTopSets * kTopThreads;
+  __shared__ TopShared<kTopThreads> s;
+  const int tid = threadIdx.x, lane = tid & 31;
   const int C = (int)cluster_size(), rank = (int)cluster_rank();
   const long r = blockIdx.x / C;
   Run<T> run = {Row<T>(logits + r * ld, V), rank * per, 0};
@@ -235,64 +214,81 @@ __global__ void __launch_bounds__(kTopThreads, 3) top_logits_kernel(const T* log
   // elements of this run, and how many of them may be among the k
   const int lo = max(run.row.column(run.first), 0), hi = min(run.row.column(run.stop), V);
   const int mine_k = min(k, max(hi - lo, 0));
+  uint4 next[kTopSets];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int j = 0; j < kTopSets; ++j) {
+      const int i = i0 + j * kTopThreads + tid;
+      if (i < run.stop) next[j] = run.row.load(i);
+    }
+  };
+  load(run.first);
   if (tid == 0) s.taken = 0;
   __syncthreads();
-  uint32_t bound = 0, top[1] = {0};                 // 16 bits of the k-th largest's lower bound, of this thread's largest
-  bool over = false;
-  int look = 1;                                     // stretches behind which the bound is raised: 1, 2, 4, ...
-  for (int i0 = run.first, n = 0; i0 < run.stop && !over; i0 += kTopAhead * kTopThreads, ++n) {
-    uint4 u[kTopAhead];
-    uint32_t t[kTopAhead];
+  constexpr int kDrop = Key<T>::kBits - 16, kShift = 32 + kDrop;
+  // a key below `least` is not among the k; k of the logits looked at so far reach the 16 bits of `bound`, and k of those in the
+  // list reach `listed`; `top` are 16 bits of this thread's largest
+  uint32_t least = 0, bound = 0, listed = 0, top = 0;
+  int look = 1;
+  for (int i0 = run.first, n = 1; i0 < run.stop; i0 += kStretch, ++n) {
+    uint4 u[kTopSets];
+    uint32_t t[kTopSets];
 #pragma unroll
-    for (int j = 0; j < kTopAhead; ++j) {
-      const int i = i0 + j * kTopThreads + tid;
-      t[j] = 0;
-      if (i < run.stop) u[j] = run.row.load(i);
-    }
+    for (int j = 0; j < kTopSets; ++j) u[j] = next[j];
+    load(i0 + kStretch);
 #pragma unroll
-    for (int j = 0; j < kTopAhead; ++j) {
-      if (i0 + j * kTopThreads + tid < run.stop) t[j] = Key<T>::top16(u[j]);
-      top[0] = max(top[0], t[j]);
+    for (int j = 0; j < kTopSets; ++j) {
+      t[j] = i0 + j * kTopThreads + tid < run.stop ? Key<T>::top16(u[j]) : 0;
+      top = max(top, t[j]);
     }
-    if (n + 1 == look) {
-      bound = kth_of_block(top, 1, k);
+    if (n == look) {
+      if (k <= kTopThreads) bound = max(bound, kth_of_block<kTopThreads>(s, top, k));
+      least = max(least, bound << kDrop);
       look *= 2;
     }
 #pragma unroll
-    for (int j = 0; j < kTopAhead; ++j) {
-      const int i = i0 + j * kTopThreads + tid;
-      if (i < run.stop && t[j] >= bound)
-        each_key<T>(run.row, i, u[j], [&](uint32_t key, int c) {
-          if (key >> (Key<T>::kBits - 16) >= bound) {
-            const int at = atomicAdd(&s.taken, 1);
-            if (at < kTopList) s.list[at] = whole_key(key, c);
-          }
-        });
+    for (int j = 0; j < kTopSets; ++j) {
+      if (i0 + j * kTopThreads >= run.stop) break;
+      // a vector that reaches the bound is looked at by a lane for each element
+      bool full = false;
+      for (uint32_t hits = __ballot_sync(0xffffffffu, t[j] >= max(least >> kDrop, 1u)); hits; hits &= hits - 1) {
+        const int l = __ffs(hits) - 1;
+        uint4 v;
+        v.x = __shfl_sync(0xffffffffu, u[j].x, l);
+        v.y = __shfl_sync(0xffffffffu, u[j].y, l);
+        v.z = __shfl_sync(0xffffffffu, u[j].z, l);
+        v.w = __shfl_sync(0xffffffffu, u[j].w, l);
+        const int c = run.row.column(i0 + j * kTopThreads + tid - lane + l) + lane;
+        const uint32_t key = Key<T>::of(element<T>(v, lane));
+        if (lane < Row<T>::kVec && c >= 0 && c < V && key >= least) {
+          const int at = atomicAdd(&s.taken, 1);    // < kTopFull + 8 * kTopThreads
+          s.list[at] = whole_key(key, c);
+          full |= at + 1 >= kTopFull;
+        }
+      }
+      if (__syncthreads_or(full)) {                 // seen by the threads that took those places: the same for all
+        rank_list<kTopThreads>(s, s.taken, k, kShift, listed, [&](int at, u64 key) { s.best[at] = key; });
+        for (int i = tid; i < k; i += kTopThreads) s.list[i] = s.best[i];
+        listed = (uint32_t)(s.best[k - 1] >> kShift);
+        least = max(least, (uint32_t)(s.best[k - 1] >> 32) + 1);
+        if (tid == 0) s.taken = k;
+        __syncthreads();
+      }
     }
-    // every stretch ends together only where the bound is raised; an overflow shows at the latest behind the last
-    if (n + 1 == look - 1 || n % 4 == 3) over = __syncthreads_or(s.taken > kTopList);
+    listed = max(listed, bound);                    // all of this stretch that reaches the bound is in the list
   }
   __syncthreads();
-  if (s.taken > kTopList) {
-    select_by_digits<T>(run, mine_k, s);
-    __syncthreads();
-    if (tid < mine_k) s.list[tid] = s.best[tid];
-    if (tid == 0) s.taken = mine_k;
-    __syncthreads();
-  }
   const int n = s.taken;
-  constexpr int kShift = 32 + Key<T>::kBits - 16;
   auto answer = [&](int at, u64 key) {
     const uint32_t c = 0xffffffffu - (uint32_t)key;
     values[r * k + at] = run.row.p[c];
     ids[r * k + at] = vocab_lo + c;
   };
   if (C == 1) {
-    rank_list(s, n, k, kShift, answer);
+    rank_list<kTopThreads>(s, n, k, kShift, listed, answer);
     return;
   }
-  rank_list(s, n, mine_k, kShift, [&](int at, u64 key) { s.best[at] = key; });
-  __syncthreads();
+  rank_list<kTopThreads>(s, n, mine_k, kShift, listed, [&](int at, u64 key) { s.best[at] = key; });
   cluster_barrier();                                // every CTA has its list
   if (rank == 0) {
     // behind one another, in the order of the CTAs
@@ -300,25 +296,37 @@ __global__ void __launch_bounds__(kTopThreads, 3) top_logits_kernel(const T* log
     for (int q = 0; q < C; ++q) {
       const int q_lo = max(run.row.column(q * per), 0), q_hi = min(run.row.column(min((q + 1) * per, run.row.vectors())), V);
       const int q_k = min(k, max(q_hi - q_lo, 0));
-      if (tid < q_k) s.list[at + tid] = cluster_load(&s.best[tid], q);
+      for (int i = tid; i < q_k; i += kTopThreads) s.list[at + i] = cluster_load(&s.best[i], q);
       at += q_k;
     }
+    // a list of k ends at a bound of the whole row's k-th largest
+    listed = 0;
+    for (int q = 0; q < C; ++q) {
+      const int q_lo = max(run.row.column(q * per), 0), q_hi = min(run.row.column(min((q + 1) * per, run.row.vectors())), V);
+      if (q_hi - q_lo >= k) listed = max(listed, (uint32_t)(cluster_load(&s.best[k - 1], q) >> kShift));
+    }
     __syncthreads();
-    rank_list(s, at, k, kShift, answer);
+    rank_list<kTopThreads>(s, at, k, kShift, listed, answer);
   }
   cluster_barrier();                                // the first CTA has read the lists
 }
 
+template <typename T, int kTopThreads>
+int launch_threads(const void* logits, void* values, long* ids, long rows, int V, long ld, int k, long vocab_lo, int C, int per,
+                   void* stream) {
+  return (int)launch_cluster(top_logits_kernel<T, kTopThreads>, (unsigned)(rows * C), kTopThreads, C, 0,
+                             VR_STREAM(stream), reinterpret_cast<const T*>(logits), reinterpret_cast<T*>(values), ids, V, ld,
+                             k, vocab_lo, per);
+}
 template <typename T>
 int launch_top(const void* logits, void* values, long* ids, long rows, int V, long ld, int k, long vocab_lo,
                void* stream) {
-  // two thirds of a wave or more: a CTA for each row; below that as many as keep a stretch of vectors each
   const long nv = ((long)V + Row<T>::kVec - 2) / Row<T>::kVec + 1;
   int C = 1;
-  while (C < kTopCluster && rows * C * 2 <= 3L * mmt_sm_count() && nv > (long)kTopThreads * C) C *= 2;
+  while (C < kTopCluster && rows * C * 2 <= 2L * mmt_sm_count() && nv > 512L * C) C *= 2;
   const int per = (int)((nv + C - 1) / C);
-  return (int)launch_cluster(top_logits_kernel<T>, (unsigned)(rows * C), kTopThreads, C, 0, VR_STREAM(stream),
-                             reinterpret_cast<const T*>(logits), reinterpret_cast<T*>(values), ids, V, ld, k, vocab_lo, per);
+  return per <= 2048 && C == 1 && k <= 64 ? launch_threads<T, 128>(logits, values, ids, rows, V, ld, k, vocab_lo, C, per, stream)
+                               : launch_threads<T, 512>(logits, values, ids, rows, V, ld, k, vocab_lo, C, per, stream);
 }
 
 }  // namespace
