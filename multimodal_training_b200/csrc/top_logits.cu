@@ -4,12 +4,16 @@
 // torch.topk has it; -0 equal to +0) above the inverted column, so that keys are unique and equal logits go by the lower
 // column.  The answer is the k largest keys of the row.
 //
-// One pass over the row, bound by memory: what is left of the logits is what reaches a lower bound of the k-th largest.  The
-// bound is the k-th largest of the threads' own largest logits so far, which are k different elements; it is raised behind
-// stretches 1, 2, 4, ... of the row, and a row in no special order leaves about k (1 + 1 + 1/2 + ...) candidates.  Where the
-// list of candidates fills up all the same (rising logits, many equal ones) it is cut to the k largest, of which the last is
-// the next bound; columns only grow, so equal logits that come later do not reach it.  In the end the candidates are cut to
-// those near the k-th largest by histograms and ranked by counting.
+// One pass over the row, bound by memory: what is left of the logits is the vectors of which an element reaches a lower bound of
+// the k-th largest.  The bound is the k-th largest of the threads' own largest logits so far, which are k different elements;
+// it is raised behind stretches 1, 2, 4, ... of the row, and a row in no special order leaves about k (1 + 1 + 1/2 + ...)
+// vectors.  Between those the warps do not wait for one another.  In the end the elements of these vectors that reach the last
+// bound, little more than k, are ranked by counting.  (Looking at the elements where a vector reaches the bound took as long as
+// the pass itself, 107 -> 226 us for 2048 x 152064 bf16 and k = 64: some lane of every third warp's load has one.)
+//
+// Where there are too many of them (rising logits, many equal ones) the run is looked at once more, step by step, and the list
+// of candidates is cut to its k largest as soon as it fills up; the last of them is the next bound, and columns only grow, so
+// equal logits that come later do not reach it.
 //
 // Few rows are cut into runs of columns, one for each CTA of a cluster; the first CTA ranks the others' lists.
 #include "vocab_rows.cuh"
@@ -23,6 +27,7 @@ constexpr int kTopSets = 4;           // vectors that a thread loads ahead: one 
 constexpr int kTopFull = 1024;        // candidates from which on the list is cut
 constexpr int kTopCluster = 8;        // most CTAs of a row; their lists fit one list: 8 * 256 = 2048
 constexpr int kTopBins = 256;
+constexpr int kTopEdge = 16;          // elements outside whole vectors, at most 7 at each end
 
 // Order-preserving bits of a logit; kBits of them.
 template <typename T>
@@ -76,20 +81,20 @@ MMT_DEVICE float element<float>(const uint4& v, int j) {
   return __uint_as_float(j & 2 ? (j & 1 ? v.w : v.z) : (j & 1 ? v.y : v.x));
 }
 
-// A CTA's run of a row: vectors [first, stop).
-template <typename T>
-struct Run {
-  Row<T> row;
-  int first, stop;
-};
-
 template <int kTopThreads>
-struct TopShared {
-  u64 list[kTopFull + 8 * kTopThreads];          // all elements of a set fit behind a list that is not full
+struct alignas(16) TopShared {
+  static constexpr int kVecs = kTopThreads < 512 ? 768 : 2048;
+  static constexpr int kStep = kTopThreads < 256 ? kTopThreads : 256;      // vectors of a step of the second look
+  static constexpr int kList = kTopFull + 8 * kStep;                      // all elements of a step fit behind a list that is not full
+  uint4 vec[kVecs];                     // vectors that reach a bound, and which they are
+  int vec_at[kVecs];
+  u64 list[kList + kTopEdge];
   u64 best[kTopMax];
   int hist[kTopBins];
+  alignas(16) uint16_t tops[kTopThreads];
+  uint32_t kth;                         // of kth_of_block
   int digit, need, count;               // of find_digit
-  int taken, kept;
+  int vecs, taken, kept;
   uint32_t warp_value[2][32];
 };
 
@@ -119,16 +124,36 @@ MMT_DEVICE uint2 range_of_block(TopShared<kTopThreads>& s, uint32_t v) {
   return make_uint2(__reduce_min_sync(0xffffffffu, s.warp_value[0][lane % (kTopThreads / 32)]),
                     __reduce_max_sync(0xffffffffu, s.warp_value[1][lane % (kTopThreads / 32)]));
 }
-// The largest t that at least k of the block's values reach; k is at most the block's size.
+// The largest t that at least k of the block's values of 16 bits reach; k is at most the block's size.  One warp searches, two
+// values an instruction.
 template <int kTopThreads>
 MMT_DEVICE uint32_t kth_of_block(TopShared<kTopThreads>& s, uint32_t v, int k) {
-  uint2 r = range_of_block<kTopThreads>(s, v);
-  while (r.x < r.y) {
-    const uint32_t at = (r.x + r.y + 1) / 2;
-    if (__syncthreads_count(v >= at) >= k) r.x = at;
-    else r.y = at - 1;
+  s.tops[threadIdx.x] = (uint16_t)v;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    constexpr int kWords = kTopThreads / 64;
+    uint32_t w[kWords], lo = 0xffffu, hi = 0;
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) {
+      w[j] = reinterpret_cast<const uint32_t*>(s.tops)[j * 32 + threadIdx.x];
+      lo = min(lo, min(w[j] & 0xffffu, w[j] >> 16));
+      hi = max(hi, max(w[j] & 0xffffu, w[j] >> 16));
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    while (lo < hi) {
+      const uint32_t at = (lo + hi + 1) / 2;
+      uint32_t count = 0;                        // of both halves
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) count += __vsetgeu2(w[j], at << 16 | at);
+      count = __reduce_add_sync(0xffffffffu, (count & 0xffffu) + (count >> 16));
+      if ((int)count >= k) lo = at;
+      else hi = at - 1;
+    }
+    if (threadIdx.x == 0) s.kth = lo;
   }
-  return r.x;
+  __syncthreads();
+  return s.kth;
 }
 // The bin at which the counts, from the last bin down, reach `need`, how many of it are needed and how many there are, into
 // shared memory.  All of the block calls it; the barrier behind it is the caller's.
@@ -156,7 +181,7 @@ MMT_DEVICE void find_digit(TopShared<kTopThreads>& s, int need) {
 template <int kTopThreads, typename F>
 MMT_DEVICE void rank_list(TopShared<kTopThreads>& s, int n, int k, int shift, uint32_t bound, F out) {
   const int tid = threadIdx.x;
-  if (n > 64 && n > k) {                          // what cannot be among the k leaves the list
+  if (n > k + 64) {                               // what cannot be among the k leaves the list
     uint32_t most = 0;
     for (int i = tid; i < n; i += kTopThreads) most = max(most, (uint32_t)(s.list[i] >> shift) & 0xffffu);
     most = range_of_block<kTopThreads>(s, most).y;
@@ -178,7 +203,7 @@ MMT_DEVICE void rank_list(TopShared<kTopThreads>& s, int n, int k, int shift, ui
       sure += need - s.need;
       need = s.need;
       const int left = sure + s.count;
-      if (left <= k + 128 || wide == 0) break;
+      if (left <= k + 64 || wide == 0) break;
       wide = max(wide - 8, 0);
       __syncthreads();                            // all have read what find_digit found
     }
@@ -204,33 +229,53 @@ __global__ void __launch_bounds__(kTopThreads, 1024 / kTopThreads) top_logits_ke
                                                                                     long* __restrict__ ids, int V, long ld,
                                                                                     int k, long vocab_lo, int per) {
   grid_dependency_sync();
-  constexpr int kStretch = kTopSets * kTopThreads;
-  __shared__ TopShared<kTopThreads> s;
-  const int tid = threadIdx.x, lane = tid & 31;
+  constexpr int kStretch = kTopSets * kTopThreads, kVec = Row<T>::kVec;
+  constexpr int kVecs = TopShared<kTopThreads>::kVecs, kStep = TopShared<kTopThreads>::kStep;
+  constexpr int kList = TopShared<kTopThreads>::kList;
+  extern __shared__ __align__(128) uint4 shared[];
+  TopShared<kTopThreads>& s = *reinterpret_cast<TopShared<kTopThreads>*>(shared);
+  const int tid = threadIdx.x;
   const int C = (int)cluster_size(), rank = (int)cluster_rank();
   const long r = blockIdx.x / C;
-  Run<T> run = {Row<T>(logits + r * ld, V), rank * per, 0};
-  run.stop = min(run.first + per, run.row.vectors());
-  // elements of this run, and how many of them may be among the k
-  const int lo = max(run.row.column(run.first), 0), hi = min(run.row.column(run.stop), V);
-  const int mine_k = min(k, max(hi - lo, 0));
+  // vectors [first, stop) of the row, whole ones [lo, hi)
+  const Row<T> row(logits + r * ld, V);
+  const int first = rank * per, stop = min(first + per, row.vectors());
+  const int lo = first + (first == 0 && row.lead != 0), hi = min(stop, (row.lead + V) / Row<T>::kVec);
+  // how many of the k this run may hold
+  auto most_of = [&](int q) {
+    const int from = max(row.column(q * per), 0), to = min(row.column(min((q + 1) * per, row.vectors())), V);
+    return min(k, max(to - from, 0));
+  };
+  const int mine_k = most_of(rank);
   uint4 next[kTopSets];
   auto load = [&](int i0) {
 #pragma unroll
     for (int j = 0; j < kTopSets; ++j) {
       const int i = i0 + j * kTopThreads + tid;
-      if (i < run.stop) next[j] = run.row.load(i);
+      if (i < hi) next[j] = *reinterpret_cast<const uint4*>(row.p + row.column(i));
     }
   };
-  load(run.first);
-  if (tid == 0) s.taken = 0;
+  load(lo);
+  if (tid == 0) s.taken = s.vecs = 0;
   __syncthreads();
   constexpr int kDrop = Key<T>::kBits - 16, kShift = 32 + kDrop;
-  // a key below `least` is not among the k; k of the logits looked at so far reach the 16 bits of `bound`, and k of those in the
-  // list reach `listed`; `top` are 16 bits of this thread's largest
-  uint32_t least = 0, bound = 0, listed = 0, top = 0;
+  // a key below `least` is not among the k; k of the logits looked at so far reach the 16 bits of `bound`; `top` are 16 bits of
+  // this thread's largest
+  uint32_t least = 0, bound = 0, top = 0;
+  auto push = [&](uint32_t key, int c) {            // whether the list is full
+    if (key < least) return false;
+    const int at = atomicAdd(&s.taken, 1);
+    if (at < kList + kTopEdge) s.list[at] = whole_key(key, c);
+    return at + 1 >= kTopFull;
+  };
+  // elements in front of the first whole vector, and behind the last one
+  auto push_edge = [&](int from, int to) {
+    if (from + tid < to) push(Key<T>::of(row.p[from + tid]), from + tid);
+  };
+  const int head = max(row.column(first), 0), head_end = min(row.column(min(lo, stop)), V);
   int look = 1;
-  for (int i0 = run.first, n = 1; i0 < run.stop; i0 += kStretch, ++n) {
+  bool over = false;
+  for (int i0 = lo, n = 1; i0 < hi && !over; i0 += kStretch, ++n) {
     uint4 u[kTopSets];
     uint32_t t[kTopSets];
 #pragma unroll
@@ -238,50 +283,68 @@ __global__ void __launch_bounds__(kTopThreads, 1024 / kTopThreads) top_logits_ke
     load(i0 + kStretch);
 #pragma unroll
     for (int j = 0; j < kTopSets; ++j) {
-      t[j] = i0 + j * kTopThreads + tid < run.stop ? Key<T>::top16(u[j]) : 0;
+      t[j] = i0 + j * kTopThreads + tid < hi ? Key<T>::top16(u[j]) : 0;
       top = max(top, t[j]);
     }
     if (n == look) {
-      if (k <= kTopThreads) bound = max(bound, kth_of_block<kTopThreads>(s, top, k));
-      least = max(least, bound << kDrop);
+      bound = kth_of_block<kTopThreads>(s, top, k);
+      over = __syncthreads_or(s.vecs > kVecs);
       look *= 2;
     }
 #pragma unroll
-    for (int j = 0; j < kTopSets; ++j) {
-      if (i0 + j * kTopThreads >= run.stop) break;
-      // a vector that reaches the bound is looked at by a lane for each element
-      bool full = false;
-      for (uint32_t hits = __ballot_sync(0xffffffffu, t[j] >= max(least >> kDrop, 1u)); hits; hits &= hits - 1) {
-        const int l = __ffs(hits) - 1;
-        uint4 v;
-        v.x = __shfl_sync(0xffffffffu, u[j].x, l);
-        v.y = __shfl_sync(0xffffffffu, u[j].y, l);
-        v.z = __shfl_sync(0xffffffffu, u[j].z, l);
-        v.w = __shfl_sync(0xffffffffu, u[j].w, l);
-        const int c = run.row.column(i0 + j * kTopThreads + tid - lane + l) + lane;
-        const uint32_t key = Key<T>::of(element<T>(v, lane));
-        if (lane < Row<T>::kVec && c >= 0 && c < V && key >= least) {
-          const int at = atomicAdd(&s.taken, 1);    // < kTopFull + 8 * kTopThreads
-          s.list[at] = whole_key(key, c);
-          full |= at + 1 >= kTopFull;
+    for (int j = 0; j < kTopSets; ++j)
+      if (t[j] >= max(bound, 1u)) {
+        const int at = atomicAdd(&s.vecs, 1);
+        if (at < kVecs) {
+          s.vec[at] = u[j];
+          s.vec_at[at] = i0 + j * kTopThreads + tid;
         }
       }
-      if (__syncthreads_or(full)) {                 // seen by the threads that took those places: the same for all
-        rank_list<kTopThreads>(s, s.taken, k, kShift, listed, [&](int at, u64 key) { s.best[at] = key; });
-        for (int i = tid; i < k; i += kTopThreads) s.list[i] = s.best[i];
-        listed = (uint32_t)(s.best[k - 1] >> kShift);
-        least = max(least, (uint32_t)(s.best[k - 1] >> 32) + 1);
-        if (tid == 0) s.taken = k;
-        __syncthreads();
-      }
-    }
-    listed = max(listed, bound);                    // all of this stretch that reaches the bound is in the list
   }
+  __syncthreads();
+  uint32_t listed = bound;                          // k of the keys in the list reach it (all, as long as there are fewer)
+  least = bound << kDrop;
+  const int vecs = s.vecs;
+  if (vecs <= kVecs) {
+    push_edge(head, head_end);
+    for (int q = tid; q < vecs * kVec; q += kTopThreads) {
+      const T x = reinterpret_cast<const T*>(s.vec)[q];
+      push(Key<T>::of(x), row.column(s.vec_at[q / kVec]) + q % kVec);
+    }
+  }
+  __syncthreads();
+  if (vecs > kVecs || s.taken > kList) {
+    __syncthreads();
+    if (tid == 0) s.taken = 0;
+    least = listed = 0;
+    __syncthreads();
+    push_edge(head, head_end);
+    for (int i0 = lo; i0 < hi; i0 += kStep) {
+      const int i = i0 + tid;
+      bool full = false;
+      if (tid < kStep && i < hi) {
+        const uint4 u = *reinterpret_cast<const uint4*>(row.p + row.column(i));
+        if (Key<T>::top16(u) >= least >> kDrop) {
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) full |= push(Key<T>::of(element<T>(u, e)), row.column(i) + e);
+        }
+      }
+      if (!__syncthreads_or(full)) continue;        // seen by the threads that took those places: the same for all
+      rank_list<kTopThreads>(s, s.taken, k, kShift, listed, [&](int at, u64 key) { s.best[at] = key; });
+      for (int q = tid; q < k; q += kTopThreads) s.list[q] = s.best[q];
+      listed = (uint32_t)(s.best[k - 1] >> kShift);
+      least = (uint32_t)(s.best[k - 1] >> 32) + 1;
+      if (tid == 0) s.taken = k;
+      __syncthreads();
+    }
+  }
+  __syncthreads();
+  push_edge(max(row.column(max(hi, lo)), 0), min(row.column(stop), V));
   __syncthreads();
   const int n = s.taken;
   auto answer = [&](int at, u64 key) {
     const uint32_t c = 0xffffffffu - (uint32_t)key;
-    values[r * k + at] = run.row.p[c];
+    values[r * k + at] = row.p[c];
     ids[r * k + at] = vocab_lo + c;
   };
   if (C == 1) {
@@ -291,19 +354,14 @@ __global__ void __launch_bounds__(kTopThreads, 1024 / kTopThreads) top_logits_ke
   rank_list<kTopThreads>(s, n, mine_k, kShift, listed, [&](int at, u64 key) { s.best[at] = key; });
   cluster_barrier();                                // every CTA has its list
   if (rank == 0) {
-    // behind one another, in the order of the CTAs
+    // behind one another, in the order of the CTAs; a list of k ends at a bound of the whole row's k-th largest
     int at = 0;
-    for (int q = 0; q < C; ++q) {
-      const int q_lo = max(run.row.column(q * per), 0), q_hi = min(run.row.column(min((q + 1) * per, run.row.vectors())), V);
-      const int q_k = min(k, max(q_hi - q_lo, 0));
-      for (int i = tid; i < q_k; i += kTopThreads) s.list[at + i] = cluster_load(&s.best[i], q);
-      at += q_k;
-    }
-    // a list of k ends at a bound of the whole row's k-th largest
     listed = 0;
     for (int q = 0; q < C; ++q) {
-      const int q_lo = max(run.row.column(q * per), 0), q_hi = min(run.row.column(min((q + 1) * per, run.row.vectors())), V);
-      if (q_hi - q_lo >= k) listed = max(listed, (uint32_t)(cluster_load(&s.best[k - 1], q) >> kShift));
+      const int q_k = most_of(q);
+      for (int i = tid; i < q_k; i += kTopThreads) s.list[at + i] = cluster_load(&s.best[i], q);
+      if (q_k == k) listed = max(listed, (uint32_t)(cluster_load(&s.best[k - 1], q) >> kShift));
+      at += q_k;
     }
     __syncthreads();
     rank_list<kTopThreads>(s, at, k, kShift, listed, answer);
@@ -314,9 +372,16 @@ __global__ void __launch_bounds__(kTopThreads, 1024 / kTopThreads) top_logits_ke
 template <typename T, int kTopThreads>
 int launch_threads(const void* logits, void* values, long* ids, long rows, int V, long ld, int k, long vocab_lo, int C, int per,
                    void* stream) {
-  return (int)launch_cluster(top_logits_kernel<T, kTopThreads>, (unsigned)(rows * C), kTopThreads, C, 0,
-                             VR_STREAM(stream), reinterpret_cast<const T*>(logits), reinterpret_cast<T*>(values), ids, V, ld,
-                             k, vocab_lo, per);
+  auto kernel = top_logits_kernel<T, kTopThreads>;
+  constexpr size_t kBytes = sizeof(TopShared<kTopThreads>);
+  static bool allowed = false;
+  if (!allowed) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBytes);
+    if (e != cudaSuccess) return (int)e;
+    allowed = true;
+  }
+  return (int)launch_cluster(kernel, (unsigned)(rows * C), kTopThreads, C, kBytes, VR_STREAM(stream),
+                             reinterpret_cast<const T*>(logits), reinterpret_cast<T*>(values), ids, V, ld, k, vocab_lo, per);
 }
 template <typename T>
 int launch_top(const void* logits, void* values, long* ids, long rows, int V, long ld, int k, long vocab_lo,
