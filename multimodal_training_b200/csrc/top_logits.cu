@@ -5,7 +5,7 @@
 // column.  The answer is the k largest keys of the row.
 //
 // One pass over the row, bound by memory: what is left of the logits is the vectors of which an element reaches a lower bound of
-// the k-th largest.  The bound is the k-th largest of the threads' own largest logits so far, which are k different elements;
+// the k-th largest.  The bound is the k-th largest of what the threads have seen as their two sets' largest, which are k different elements;
 // it is raised behind stretches 1, 2, 4, ... of the row, and a row in no special order leaves about k (1 + 1 + 1/2 + ...)
 // vectors.  Between those the warps do not wait for one another.  In the end the elements of these vectors that reach the last
 // bound, little more than k, are ranked by counting.  (Looking at the elements where a vector reaches the bound took as long as
@@ -41,6 +41,11 @@ struct Key<bf16> {
     if (b == 0x8000u) b = 0;
     return b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
   }
+  // The logit of a key, if the key tells.
+  static MMT_DEVICE bool back(uint32_t key, bf16& x) {
+    x = __ushort_as_bfloat16((unsigned short)(key & 0x8000u ? key & 0x7fffu : ~key));
+    return key != 0x8000u && key != 0xffffu;
+  }
   // Bits of the largest element of a vector that bound a thread's largest from below, as of() orders them; 16 of them.
   static MMT_DEVICE uint32_t top16(const uint4& u) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -58,6 +63,10 @@ struct Key<float> {
     if ((b & 0x7fffffffu) > 0x7f800000u) return 0xfffffffeu;          // one below the largest: there is a key above it
     if (b == 0x80000000u) b = 0;
     return b & 0x80000000u ? ~b : b | 0x80000000u;
+  }
+  static MMT_DEVICE bool back(uint32_t key, float& x) {
+    x = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+    return key != 0x80000000u && key != 0xfffffffeu;
   }
   static MMT_DEVICE uint32_t top16(const uint4& u) {
     const float v[4] = {__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w)};
@@ -83,16 +92,14 @@ MMT_DEVICE float element<float>(const uint4& v, int j) {
 
 template <int kTopThreads>
 struct alignas(16) TopShared {
-  static constexpr int kVecs = kTopThreads < 512 ? 768 : 2048;
+  static constexpr int kVecs = kTopThreads == 128 ? 768 : kTopThreads == 256 ? 1536 : 2048;
   static constexpr int kStep = kTopThreads < 256 ? kTopThreads : 256;      // vectors of a step of the second look
   static constexpr int kList = kTopFull + 8 * kStep;                      // all elements of a step fit behind a list that is not full
   uint4 vec[kVecs];                     // vectors that reach a bound, and which they are
   int vec_at[kVecs];
-  u64 list[kList + kTopEdge];
+  alignas(16) u64 list[kList + kTopEdge];
   u64 best[kTopMax];
   int hist[kTopBins];
-  alignas(16) uint16_t tops[kTopThreads];
-  uint32_t kth;                         // of kth_of_block
   int digit, need, count;               // of find_digit
   int vecs, taken, kept;
   uint32_t warp_value[2][32];
@@ -110,11 +117,12 @@ MMT_DEVICE int up_to_lane(int v) {
   }
   return v;
 }
-// Smallest and largest of a block's values.
+// Smallest and largest of a block's values, of which each thread has its own smallest and largest.
 template <int kTopThreads>
-MMT_DEVICE uint2 range_of_block(TopShared<kTopThreads>& s, uint32_t v) {
+MMT_DEVICE uint2 range_of_block(TopShared<kTopThreads>& s, uint32_t lo, uint32_t hi) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t lo = __reduce_min_sync(0xffffffffu, v), hi = __reduce_max_sync(0xffffffffu, v);
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
   __syncthreads();
   if (lane == 0) {
     s.warp_value[0][warp] = lo;
@@ -123,37 +131,6 @@ MMT_DEVICE uint2 range_of_block(TopShared<kTopThreads>& s, uint32_t v) {
   __syncthreads();
   return make_uint2(__reduce_min_sync(0xffffffffu, s.warp_value[0][lane % (kTopThreads / 32)]),
                     __reduce_max_sync(0xffffffffu, s.warp_value[1][lane % (kTopThreads / 32)]));
-}
-// The largest t that at least k of the block's values of 16 bits reach; k is at most the block's size.  One warp searches, two
-// values an instruction.
-template <int kTopThreads>
-MMT_DEVICE uint32_t kth_of_block(TopShared<kTopThreads>& s, uint32_t v, int k) {
-  s.tops[threadIdx.x] = (uint16_t)v;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    constexpr int kWords = kTopThreads / 64;
-    uint32_t w[kWords], lo = 0xffffu, hi = 0;
-#pragma unroll
-    for (int j = 0; j < kWords; ++j) {
-      w[j] = reinterpret_cast<const uint32_t*>(s.tops)[j * 32 + threadIdx.x];
-      lo = min(lo, min(w[j] & 0xffffu, w[j] >> 16));
-      hi = max(hi, max(w[j] & 0xffffu, w[j] >> 16));
-    }
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    hi = __reduce_max_sync(0xffffffffu, hi);
-    while (lo < hi) {
-      const uint32_t at = (lo + hi + 1) / 2;
-      uint32_t count = 0;                        // of both halves
-#pragma unroll
-      for (int j = 0; j < kWords; ++j) count += __vsetgeu2(w[j], at << 16 | at);
-      count = __reduce_add_sync(0xffffffffu, (count & 0xffffu) + (count >> 16));
-      if ((int)count >= k) lo = at;
-      else hi = at - 1;
-    }
-    if (threadIdx.x == 0) s.kth = lo;
-  }
-  __syncthreads();
-  return s.kth;
 }
 // The bin at which the counts, from the last bin down, reach `need`, how many of it are needed and how many there are, into
 // shared memory.  All of the block calls it; the barrier behind it is the caller's.
@@ -176,6 +153,25 @@ MMT_DEVICE void find_digit(TopShared<kTopThreads>& s, int need) {
   }
 }
 
+// A t that at least k of the block's values, two a thread, reach: near the largest one, the lower end of its bin in a histogram
+// of their range above `least` (a t from before) and, 16 bits having 128 values between two powers of two, of eight powers of
+// two below the largest value.  `least` if fewer than k values are in that range.
+template <int kTopThreads>
+MMT_DEVICE uint32_t kth_of_block(TopShared<kTopThreads>& s, const uint32_t (&v)[2], int k, uint32_t least) {
+  for (int b = threadIdx.x; b < kTopBins; b += kTopThreads) s.hist[b] = 0;
+  if (threadIdx.x == 0) s.digit = -1;
+  uint2 r = range_of_block<kTopThreads>(s, min(v[0] - 1u, v[1] - 1u), max(v[0], v[1]));      // 0 is none
+  r.x = max(max(r.x + 1u, least), r.y > 1023u ? r.y - 1023u : 1u);
+  const int wide = r.y < r.x ? 0 : 32 - __clz((r.y - r.x) / kTopBins);
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (v[j] >= r.x) atomicAdd(&s.hist[(v[j] - r.x) >> wide], 1);
+  __syncthreads();
+  find_digit(s, k);
+  __syncthreads();
+  return s.digit < 0 ? least : r.x + ((uint32_t)s.digit << wide);
+}
+
 // Ranks the n keys of the list and hands out the k largest: out(rank, key).  n >= k, and k of the keys reach `bound` (16 bits
 // from `shift` up).  All threads come out of it together.
 template <int kTopThreads, typename F>
@@ -184,7 +180,7 @@ MMT_DEVICE void rank_list(TopShared<kTopThreads>& s, int n, int k, int shift, ui
   if (n > k + 64) {                               // what cannot be among the k leaves the list
     uint32_t most = 0;
     for (int i = tid; i < n; i += kTopThreads) most = max(most, (uint32_t)(s.list[i] >> shift) & 0xffffu);
-    most = range_of_block<kTopThreads>(s, most).y;
+    most = range_of_block<kTopThreads>(s, most, most).y;
     // keys in [low, low + bins) compete for `need` places; those above have theirs
     u64 low = (u64)bound << shift;
     int wide = shift + 32 - __clz((most - bound) / kTopBins), need = k, sure = 0;
@@ -215,10 +211,16 @@ MMT_DEVICE void rank_list(TopShared<kTopThreads>& s, int n, int k, int shift, ui
     }
     n = s.kept;
   }
+  if (tid == 0) s.list[n] = 0;                    // for the last pair
+  __syncthreads();
   for (int i = tid; i < n; i += kTopThreads) {
     const u64 key = s.list[i];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += s.list[j] > key;
+#pragma unroll 4
+    for (int j = 0; j < n; j += 2) {
+      const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&s.list[j]);
+      rank += (v.x > key) + (v.y > key);
+    }
     if (rank < k) out(rank, key);
   }
   __syncthreads();
@@ -260,8 +262,8 @@ __global__ void __launch_bounds__(kTopThreads, 1024 / kTopThreads) top_logits_ke
   __syncthreads();
   constexpr int kDrop = Key<T>::kBits - 16, kShift = 32 + kDrop;
   // a key below `least` is not among the k; k of the logits looked at so far reach the 16 bits of `bound`; `top` are 16 bits of
-  // this thread's largest
-  uint32_t least = 0, bound = 0, top = 0;
+  // this thread's largest of the even and the odd sets
+  uint32_t least = 0, bound = 0, top[2] = {0, 0};
   auto push = [&](uint32_t key, int c) {            // whether the list is full
     if (key < least) return false;
     const int at = atomicAdd(&s.taken, 1);
@@ -284,10 +286,10 @@ __global__ void __launch_bounds__(kTopThreads, 1024 / kTopThreads) top_logits_ke
 #pragma unroll
     for (int j = 0; j < kTopSets; ++j) {
       t[j] = i0 + j * kTopThreads + tid < hi ? Key<T>::top16(u[j]) : 0;
-      top = max(top, t[j]);
+      top[j % 2] = max(top[j % 2], t[j]);
     }
     if (n == look) {
-      bound = kth_of_block<kTopThreads>(s, top, k);
+      bound = kth_of_block<kTopThreads>(s, top, k, bound);
       over = __syncthreads_or(s.vecs > kVecs);
       look *= 2;
     }
@@ -344,7 +346,10 @@ __global__ void __launch_bounds__(kTopThreads, 1024 / kTopThreads) top_logits_ke
   const int n = s.taken;
   auto answer = [&](int at, u64 key) {
     const uint32_t c = 0xffffffffu - (uint32_t)key;
-    values[r * k + at] = row.p[c];
+    T x;
+    // zeros and NaN have lost bits in their keys
+    if (!Key<T>::back((uint32_t)(key >> 32), x)) x = row.p[c];
+    values[r * k + at] = x;
     ids[r * k + at] = vocab_lo + c;
   };
   if (C == 1) {
@@ -387,10 +392,15 @@ template <typename T>
 int launch_top(const void* logits, void* values, long* ids, long rows, int V, long ld, int k, long vocab_lo,
                void* stream) {
   const long nv = ((long)V + Row<T>::kVec - 2) / Row<T>::kVec + 1;
+  // few rows: up to two CTAs an SM, as long as a CTA has a vector for each thread
   int C = 1;
   while (C < kTopCluster && rows * C * 2 <= 2L * mmt_sm_count() && nv > 512L * C) C *= 2;
   const int per = (int)((nv + C - 1) / C);
-  return per <= 2048 && C == 1 && k <= 64 ? launch_threads<T, 128>(logits, values, ids, rows, V, ld, k, vocab_lo, C, per, stream)
+  // Short rows have few stretches, and more of them fit an SM in smaller CTAs; a large k needs many values for its bound.
+  // 4096 x 5000 bf16, k = 64: 34 us with 128 threads, 43 with 256, 62 with 512; 4096 x 2000 fp32, k = 256: 111, 105, 123;
+  // 1024 x 152064 bf16, k = 256: 486, 196, 94.
+  if (per <= 2048 && C == 1 && k <= 64) return launch_threads<T, 128>(logits, values, ids, rows, V, ld, k, vocab_lo, C, per, stream);
+  return per <= 4096 && C == 1 ? launch_threads<T, 256>(logits, values, ids, rows, V, ld, k, vocab_lo, C, per, stream)
                                : launch_threads<T, 512>(logits, values, ids, rows, V, ld, k, vocab_lo, C, per, stream);
 }
 
