@@ -335,58 +335,9 @@ __global__ void __launch_bounds__(kDistillThreads) distill_grad_kernel(const T* 
 // ----------------------------------------------------------------------------
 constexpr int kSingle = 0, kSquares = 1, kTwice = 2;
 
-MMT_DEVICE float pow2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-MMT_DEVICE float thread_max(const uint4& u, float m, bf16) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-  __nv_bfloat162 t = *reinterpret_cast<const __nv_bfloat162*>(&w[0]);
-#pragma unroll
-  for (int j = 1; j < 4; ++j) t = __hmax2(t, *reinterpret_cast<const __nv_bfloat162*>(&w[j]));
-  return fmaxf(m, fmaxf(__low2float(t), __high2float(t)));
-}
-MMT_DEVICE float thread_max(const uint4& u, float m, float) {
-  return fmaxf(fmaxf(m, fmaxf(__uint_as_float(u.x), __uint_as_float(u.y))),
-               fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
-}
-// Largest of a warp's values, NaN left out.
-MMT_DEVICE float warp_top(float v) {
-  float r;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
-}
 // 2^(a - b) for two tops, 0 for a set without any mass.
 MMT_DEVICE float rescale(float m, float c, float top) { return m == -INFINITY ? 0.f : pow2(__fmul_rn(m, c) - top); }
 
-// Two fp32 values in one 64-bit register: an instruction works on both.
-typedef unsigned long long f32x2;
-MMT_DEVICE f32x2 both(float lo, float hi) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-MMT_DEVICE float2 apart(f32x2 v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-MMT_DEVICE f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-MMT_DEVICE f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-MMT_DEVICE f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // The two powers of two logits, with c = (c, c) and so on.
 struct Powers {
   f32x2 c, c1, less, less1;               // less = (-top, -top)

@@ -29,67 +29,6 @@ constexpr int kTopCluster = 8;        // most CTAs of a row; their lists fit one
 constexpr int kTopBins = 256;
 constexpr int kTopEdge = 16;          // elements outside whole vectors, at most 7 at each end
 
-// Order-preserving bits of a logit; kBits of them.
-template <typename T>
-struct Key;
-template <>
-struct Key<bf16> {
-  static constexpr int kBits = 16;
-  static MMT_DEVICE uint32_t of(bf16 x) {
-    uint32_t b = __bfloat16_as_ushort(x);
-    if ((b & 0x7fffu) > 0x7f80u) return 0xffffu;
-    if (b == 0x8000u) b = 0;
-    return b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
-  }
-  // The logit of a key, if the key tells.
-  static MMT_DEVICE bool back(uint32_t key, bf16& x) {
-    x = __ushort_as_bfloat16((unsigned short)(key & 0x8000u ? key & 0x7fffu : ~key));
-    return key != 0x8000u && key != 0xffffu;
-  }
-  // Bits of the largest element of a vector that bound a thread's largest from below, as of() orders them; 16 of them.
-  static MMT_DEVICE uint32_t top16(const uint4& u) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    __nv_bfloat162 t = *reinterpret_cast<const __nv_bfloat162*>(&w[0]);
-#pragma unroll
-    for (int j = 1; j < 4; ++j) t = __hmax2_nan(t, *reinterpret_cast<const __nv_bfloat162*>(&w[j]));
-    return of(__hmax_nan(__low2bfloat16(t), __high2bfloat16(t)));
-  }
-};
-template <>
-struct Key<float> {
-  static constexpr int kBits = 32;
-  static MMT_DEVICE uint32_t of(float x) {
-    uint32_t b = __float_as_uint(x);
-    if ((b & 0x7fffffffu) > 0x7f800000u) return 0xfffffffeu;          // one below the largest: there is a key above it
-    if (b == 0x80000000u) b = 0;
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
-  }
-  static MMT_DEVICE bool back(uint32_t key, float& x) {
-    x = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
-    return key != 0x80000000u && key != 0xfffffffeu;
-  }
-  static MMT_DEVICE uint32_t top16(const uint4& u) {
-    const float v[4] = {__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w)};
-    uint32_t t = of(v[0]);
-#pragma unroll
-    for (int j = 1; j < 4; ++j) t = max(t, of(v[j]));
-    return t >> 16;
-  }
-};
-
-// Element j (of as many as a vector has) of a vector.
-template <typename T>
-MMT_DEVICE T element(const uint4& v, int j);
-template <>
-MMT_DEVICE bf16 element<bf16>(const uint4& v, int j) {
-  const uint32_t w = j & 4 ? (j & 2 ? v.w : v.z) : (j & 2 ? v.y : v.x);
-  return __ushort_as_bfloat16((unsigned short)(j & 1 ? w >> 16 : w));
-}
-template <>
-MMT_DEVICE float element<float>(const uint4& v, int j) {
-  return __uint_as_float(j & 2 ? (j & 1 ? v.w : v.z) : (j & 1 ? v.y : v.x));
-}
-
 template <int kTopThreads>
 struct alignas(16) TopShared {
   static constexpr int kVecs = kTopThreads == 128 ? 768 : kTopThreads == 256 ? 1536 : 2048;

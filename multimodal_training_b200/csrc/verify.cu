@@ -7,13 +7,20 @@
 // whose cumulative weight exceeds r times the total.  tau = 0: x_i is accepted while it is the largest logit's id (equal
 // logits: the lowest id, NaN above everything), and the next token is that id of row a.
 //
-// A drawn token depends on a sum over the whole vocabulary that may end next to a border, so probabilities and sums are
-// fp64: an error e of the cumulative weights gives another token with probability 2 V e.
+// A drawn token depends on a sum over the whole vocabulary that may end next to a border: an error e of the cumulative
+// weights gives another token with probability 2 V e.  So the row that is drawn from is weighed in fp64.  The normalisers of
+// all rows, one pass over memory, are fp32 sums; their error is below 2^-15 (a thread adds up to 300 terms one by one), so a
+// draft whose acceptance that could change has its two rows summed again in fp64.
 #include "vocab_rows.cuh"
 
 namespace {
 
-constexpr int kVerifyThreads = 512;
+constexpr int kRowThreads = 256;                  // of a CTA that reads a part of a row
+constexpr int kRowAhead = 4;                      // vectors that a thread loads before it works on them
+constexpr int kDrawThreads = 256;
+constexpr int kDrawWarps = kDrawThreads / 32;
+constexpr int kDrawCluster = 8;                   // CTAs that weigh a row
+constexpr double kLog2e = 1.44269504088896340736;
 
 struct Verify {
   const void* target;                 // [batch, drafts + 1, V]
@@ -25,10 +32,11 @@ struct Verify {
   long* accepted;                     // [batch]
   long* tokens;                       // [batch, drafts + 1]
   float* accept_prob;                 // [batch, drafts]
-  double* stats;                      // [batch, 2 drafts + 1, 2]: largest logit and sum of exp((x - largest) / tau);
-                                      // without sampling the id of the largest logit
+  unsigned long long* parts;          // [batch, rows, splits]: (largest logit, sum of 2^(x c - fl(largest c))) of each part of
+                                      // a row; without sampling the key of its largest logit
   double inv_temperature;
   int batch, drafts, V, is_f32, uniforms_f64, sampled;
+  int rows, splits;                   // rows of a sequence (the target's, then the draft model's), parts of a row
 };
 
 MMT_DEVICE int draft_len(const Verify& v, int b) {
@@ -49,196 +57,472 @@ template <typename T>
 MMT_DEVICE Row<T> draft_row(const Verify& v, int b, int i) {
   return Row<T>(reinterpret_cast<const T*>(v.draft) + b * v.draft_seq + i * v.draft_row, v.V);
 }
-MMT_DEVICE double weight(float x, double top, double inv_temperature) {
-  return exp(((double)x - top) * inv_temperature);
-}
+// fp32 exponents are x c - fl(m c), as in the sums of csrc/distill.cu.
+MMT_DEVICE float scale_of(const Verify& v) { return (float)(kLog2e * v.inv_temperature); }
 
 // ----------------------------------------------------------------------------
-// Rows: largest logit and normaliser, or the id of the largest logit.  One CTA per row: the drafts + 1 of the target, then
-// those of the draft model.
+// Rows: (largest logit, sum), or the key of the largest logit, of each part of a row.
 // ----------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(kVerifyThreads) verify_rows_kernel(Verify v) {
+MMT_DEVICE unsigned long long key_of(T x, int c) {
+  return (unsigned long long)Key<T>::of(x) << 32 | (0xffffffffu - (uint32_t)c);
+}
+
+template <typename T, bool kSampled>
+__global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(Verify v) {
   grid_dependency_sync();
-  __shared__ float red[kVerifyThreads / 32];
-  __shared__ double dred[kVerifyThreads / 32];
-  const int b = blockIdx.y, r = blockIdx.x, len = draft_len(v, b);
+  constexpr int kVec = Row<T>::kVec, kWarps = kRowThreads / 32;
+  __shared__ float2 warp_part[kWarps];
+  __shared__ unsigned long long warp_key[kWarps];
+  const int b = blockIdx.z, r = blockIdx.y, len = draft_len(v, b);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const bool of_target = r <= v.drafts;
   if (of_target ? r > len : r - v.drafts - 1 >= len) return;
   const Row<T> row = of_target ? target_row<T>(v, b, r) : draft_row<T>(v, b, r - v.drafts - 1);
-  const int nv = row.vectors();
-  double* out = v.stats + ((long)b * (2 * v.drafts + 1) + r) * 2;
-  float m = -INFINITY;
-  bool nan = false;
-  for (int i = threadIdx.x; i < nv; i += kVerifyThreads) {
-    float x[Row<T>::kVec];
-    RowVec<T>::unpack(row.load(i), x);
+  // vectors [first, stop) of the row, whole ones [lo, hi); `edge`: a column outside the whole ones for each of a few threads
+  const int nv = row.vectors(), per = (nv + v.splits - 1) / v.splits;
+  const int first = blockIdx.x * per, stop = min(first + per, nv);
+  const int lo = first + (first == 0 && row.lead != 0), hi = max(lo, min(stop, (row.lead + v.V) / kVec));
+  int edge = -1;
+  if (first < stop) {
+    const int head = max(row.column(first), 0), head_end = min(row.column(min(lo, stop)), v.V);
+    const int tail = max(row.column(hi), 0), tail_end = min(row.column(stop), v.V);
+    if (head + tid < head_end) edge = head + tid;
+    else if (tid >= kVec && tail + tid - kVec < tail_end) edge = tail + tid - kVec;
+  }
+  unsigned long long* out = v.parts + ((long)b * v.rows + r) * v.splits + blockIdx.x;
+
+  if constexpr (!kSampled) {
+    // a thread's largest vector, the first of several; its element is looked up in the end
+    uint32_t top = 0;
+    int at = -1;
+    for (int i0 = lo + tid; i0 < hi; i0 += kRowAhead * kRowThreads) {
+      uint4 u[kRowAhead];
 #pragma unroll
-    for (int j = 0; j < Row<T>::kVec; ++j) {
-      m = fmaxf(m, x[j]);
-      nan |= !(x[j] == x[j]);
+      for (int k = 0; k < kRowAhead; ++k)
+        if (i0 + k * kRowThreads < hi) u[k] = *reinterpret_cast<const uint4*>(row.p + row.column(i0 + k * kRowThreads));
+#pragma unroll
+      for (int k = 0; k < kRowAhead; ++k) {
+        const int i = i0 + k * kRowThreads;
+        const uint32_t t = i < hi ? Key<T>::top(u[k]) : 0;
+        if (t > top) {
+          top = t;
+          at = i;
+        }
+      }
     }
-  }
-  m = block_top<kVerifyThreads>(m, red);
-  if (!v.sampled) {
-    nan = __syncthreads_or(nan);
-    __shared__ int first;
-    if (threadIdx.x == 0) first = v.V;
-    __syncthreads();
-    int mine = v.V;
-    for (int i = threadIdx.x; i < nv && mine == v.V; i += kVerifyThreads) {
-      float x[Row<T>::kVec];
-      RowVec<T>::unpack(row.load(i), x);
-      const int c = row.column(i);
+    unsigned long long key = edge >= 0 ? key_of(row.p[edge], edge) : 0;
+    if (at >= 0) {
 #pragma unroll
-      for (int j = Row<T>::kVec - 1; j >= 0; --j)
-        if (c + j >= 0 && c + j < v.V && (nan ? !(x[j] == x[j]) : x[j] == m)) mine = c + j;
+      for (int j = 0; j < kVec; ++j) key = max(key, key_of(row.p[row.column(at) + j], row.column(at) + j));
     }
-    if (mine < v.V) atomicMin(&first, mine);
-    __syncthreads();
-    if (threadIdx.x == 0) out[0] = (double)first;
-    return;
-  }
-  double s = 0.0;
-  for (int i = threadIdx.x; i < nv; i += kVerifyThreads) {
-    float x[Row<T>::kVec];
-    RowVec<T>::unpack(row.load(i), x);
-    const int c = row.column(i);
 #pragma unroll
-    for (int j = 0; j < Row<T>::kVec; ++j)
-      if (c + j >= 0 && c + j < v.V) s += weight(x[j], (double)m, v.inv_temperature);
-  }
-  s = block_total<kVerifyThreads>(s, dred);
-  if (threadIdx.x == 0) {
-    out[0] = (double)m;
-    out[1] = s;
+    for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+    if (lane == 0) warp_key[warp] = key;
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) key = max(key, warp_key[w]);
+      *out = key;
+    }
+  } else {
+    const float c = scale_of(v);
+    const f32x2 c2 = both(c, c);
+    float m = edge >= 0 ? to_float(row.p[edge]) : -INFINITY;
+    const float x0 = m;
+    m = warp_top(m);
+    float t = m == -INFINITY ? 0.f : __fmul_rn(m, c);
+    // what is not a number makes the sum so, and a warp that has nothing but -inf adds zeros (2^-inf), not 2^(-inf + inf)
+    f32x2 s = both(edge >= 0 ? pow2(__fmaf_rn(x0, c, -t)) : 0.f, 0.f);
+    for (int i0 = lo + warp * 32; i0 < hi; i0 += kRowAhead * kRowThreads) {
+      uint4 u[kRowAhead];
+      const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+#pragma unroll
+      for (int k = 0; k < kRowAhead; ++k) {
+        const int i = i0 + k * kRowThreads + lane;
+        u[k] = make_uint4(none, none, none, none);
+        if (i < hi) u[k] = *reinterpret_cast<const uint4*>(row.p + row.column(i));
+      }
+      float top = m;
+#pragma unroll
+      for (int k = 0; k < kRowAhead; ++k) top = thread_max(u[k], top, T());
+      top = warp_top(top);
+      if (top > m) {
+        const float less = __fmul_rn(top, c), by = m == -INFINITY ? 0.f : pow2(t - less);
+        s = mul2(s, both(by, by));
+        t = less;
+        m = top;
+      }
+      const f32x2 less2 = both(-t, -t);
+#pragma unroll
+      for (int k = 0; k < kRowAhead; ++k) {
+        float x[kVec];
+        RowVec<T>::unpack(u[k], x);
+#pragma unroll
+        for (int j = 0; j < kVec; j += 2) {
+          const float2 e = apart(fma2(both(x[j], x[j + 1]), c2, less2));
+          s = add2(s, both(pow2(e.x), pow2(e.y)));
+        }
+      }
+    }
+    const float sum = warp_sum(apart(s).x + apart(s).y);
+    if (lane == 0) warp_part[warp] = make_float2(m, sum);
+    __syncthreads();
+    if (warp == 0) {
+      const float2 a = warp_part[lane % kWarps];
+      const float top = warp_top(a.x), less = __fmul_rn(top, c);
+      float part = a.x == -INFINITY ? a.y : a.y * pow2(__fmul_rn(a.x, c) - less);
+#pragma unroll
+      for (int o = kWarps / 2; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+      if (lane == 0) *reinterpret_cast<float2*>(out) = make_float2(top, part);
+    }
   }
 }
 
-// Accepted drafts of a sequence; the first `drafts` entries of accept_prob and the tokens but the drawn one.
+// ----------------------------------------------------------------------------
+// Sequences.  The first CTA of a sequence's cluster writes its answers.
+// ----------------------------------------------------------------------------
+struct DrawShared {
+  double table[64];                   // 2^(i / 64)
+  double warp_total[kDrawWarps];
+  float4 cta_part[2][kDrawCluster];   // two doubles each
+  int first, first_sure;
+};
+
+// 2^(z / 64) in fp64 from a table and a polynomial (Tang, Table-driven implementation of the exponential function, 1989):
+// z = n + f with a whole n and |f| <= 1/2, 2^(n / 64) from the table and the exponent, 2^(f / 64) to 2^-54 by its series.
+MMT_DEVICE double exp2_64th(double z, const double* table) {
+  if (!(z > -64.0 * 1000.0)) return z == z ? 0.0 : z;
+  constexpr double kMagic = 6755399441055744.0;                  // 1.5 * 2^52: adding it rounds to a whole number
+  constexpr double kLn = 0.69314718055994530942 / 64.0;
+  const double shifted = z + kMagic, f = z - (shifted - kMagic);
+  const int n = __double2loint(shifted);
+  double p = fma(kLn * kLn * kLn * kLn * kLn / 120.0, f, kLn * kLn * kLn * kLn / 24.0);
+  p = fma(p, f, kLn * kLn * kLn / 6.0);
+  p = fma(p, f, kLn * kLn / 2.0);
+  p = fma(p, f, kLn);
+  p *= f;
+  const double t = table[n & 63], e = fma(t, p, t);
+  return __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
+}
+
+// Weights of the columns of a row that a token is drawn from.
+enum Draw { kPlain, kWithout, kRest };            // p; p without one id; max(p - q, 0)
 template <typename T>
-MMT_DEVICE int accept(const Verify& v, int b, int len, int* first) {
-  if (threadIdx.x == 0) *first = len;
+struct Weigher {
+  Row<T> p;
+  const T* q;
+  const double* table;
+  double scale, less_p, less_q, by_p, by_q;       // exponents x scale - less in 64ths, times by
+  long x;
+  Draw kind;
+  MMT_DEVICE double of(T xp, int c) const {
+    const double e = exp2_64th(fma((double)to_float(xp), scale, -less_p), table);
+    if (kind == kPlain) return e;
+    if (kind == kWithout) return c == x ? 0.0 : e;
+    const double d = e * by_p - exp2_64th(fma((double)to_float(q[c]), scale, -less_q), table) * by_q;
+    return d > 0.0 ? d : d == d ? 0.0 : d;
+  }
+  // Sum over vector i, whose logits are `u` if it is a whole one.
+  MMT_DEVICE double sum(int i, const uint4& u) const {
+    const int c = p.column(i);
+    double s = 0.0;
+    if (p.whole(i)) {
+      uint4 uq = u;
+      const bool pair = kind == kRest && Row<T>::lead_of(q) == p.lead;
+      if (pair) uq = *reinterpret_cast<const uint4*>(q + c);
+#pragma unroll
+      for (int j = 0; j < Row<T>::kVec; ++j) {
+        if (pair) {
+          const double d = exp2_64th(fma((double)to_float(element<T>(u, j)), scale, -less_p), table) * by_p -
+                           exp2_64th(fma((double)to_float(element<T>(uq, j)), scale, -less_q), table) * by_q;
+          s += d > 0.0 ? d : d == d ? 0.0 : d;
+        } else {
+          s += of(element<T>(u, j), c + j);
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int j = 0; j < Row<T>::kVec; ++j)
+        if (c + j >= 0 && c + j < p.V) s += of(p.p[c + j], c + j);
+    }
+    return s;
+  }
+  // Sum over the vectors from `i` on in steps of `step`, below `stop`.
+  MMT_DEVICE double sum_run(int i, int stop, int step) const {
+    double s = 0.0;
+    uint4 next = make_uint4(0u, 0u, 0u, 0u);
+    if (i < stop && p.whole(i)) next = *reinterpret_cast<const uint4*>(p.p + p.column(i));
+    for (; i < stop; i += step) {
+      const uint4 u = next;
+      if (i + step < stop && p.whole(i + step)) next = *reinterpret_cast<const uint4*>(p.p + p.column(i + step));
+      s += sum(i, u);
+    }
+    return s;
+  }
+};
+
+MMT_DEVICE double warp_total_of(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(Verify v) {
+  grid_dependency_sync();
+  __shared__ DrawShared s;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int C = (int)cluster_size(), rank = (int)cluster_rank();
+  const int b = blockIdx.x / C, n = v.drafts, len = draft_len(v, b);
+  const long at = (long)b * (n + 1);
+  if (tid < 64) s.table[tid] = exp2((double)tid / 64.0);
+  if (tid == 0) s.first = s.first_sure = len;
   __syncthreads();
-  const double* st = v.stats + (long)b * (2 * v.drafts + 1) * 2;
-  for (int i = threadIdx.x; i < v.drafts; i += kVerifyThreads) {
+  cluster_barrier();                               // every CTA has started: its shared memory may be written
+  int turn = 0;
+  const double scale = 64.0 * kLog2e * v.inv_temperature;
+
+  // largest logit and normaliser of a row, from its parts
+  const float c = scale_of(v);
+  auto row_sum = [&](int r) {
+    const float2* part = reinterpret_cast<const float2*>(v.parts + ((long)b * v.rows + r) * v.splits);
+    float m = part[0].x;
+    for (int k = 1; k < v.splits; ++k) m = fmaxf(m, part[k].x);
+    double sum = 0.0;
+    for (int k = 0; k < v.splits; ++k) {
+      const float2 a = part[k];
+      // the part's sum is relative to fl(its largest c)
+      const double by = a.x == -INFINITY ? 1.0 : exp2((double)__fmul_rn(a.x, c) - (double)m * (double)c);
+      sum += (double)a.y * by;
+    }
+    return make_double2((double)m, sum);
+  };
+  // a value of each CTA, summed in their order
+  auto cluster_total = [&](double2 mine) {
+    if (tid < C) {
+      float4 w;
+      *reinterpret_cast<double2*>(&w) = mine;
+      cluster_store(&s.cta_part[turn][rank], tid, w);
+    }
+    cluster_barrier();
+    double2 total = make_double2(0.0, 0.0);
+    for (int k = 0; k < C; ++k) {
+      const double2 a = *reinterpret_cast<const double2*>(&s.cta_part[turn][k]);
+      total.x += a.x;
+      total.y += a.y;
+    }
+    turn ^= 1;
+    return total;
+  };
+  auto block_sum = [&](double x) {
+    x = warp_total_of(x);
+    __syncthreads();
+    if (lane == 0) s.warp_total[warp] = x;
+    __syncthreads();
+    double t = 0.0;
+#pragma unroll
+    for (int w = 0; w < kDrawWarps; ++w) t += s.warp_total[w];
+    return t;
+  };
+  // this CTA's run of a row's vectors
+  auto run_of = [&](const Row<T>& row) {
+    const int nv = row.vectors(), per = (nv + C - 1) / C;
+    return make_int2(min(rank * per, nv), min((rank + 1) * per, nv));
+  };
+  // normalisers of a row of the target and of the draft model, in fp64
+  auto exact_sums = [&](int i, bool with_q, double m_p, double m_q) {
+    Weigher<T> w = {target_row<T>(v, b, i), nullptr, s.table, scale, m_p * scale, 0.0, 1.0, 1.0, -1, kPlain};
+    int2 run = run_of(w.p);
+    const double sum_p = block_sum(w.sum_run(run.x + tid, run.y, kDrawThreads));
+    double sum_q = 0.0;
+    if (with_q) {
+      w.p = draft_row<T>(v, b, i);
+      w.less_p = m_q * scale;
+      run = run_of(w.p);
+      sum_q = block_sum(w.sum_run(run.x + tid, run.y, kDrawThreads));
+    }
+    return cluster_total(make_double2(sum_p, sum_q));
+  };
+
+  // ---- acceptance: every CTA decides for itself
+  for (int i = tid; i < n; i += kDrawThreads) {
     float prob = 0.f;
     if (i < len) {
-      const long x = v.draft_ids[(long)b * v.drafts + i];
-      bool ok;
+      const long x = v.draft_ids[(long)b * n + i];
       if (!v.sampled) {
-        ok = (double)x == st[2 * i];
+        const unsigned long long* part = v.parts + ((long)b * v.rows + i) * v.splits;
+        unsigned long long key = part[0];
+        for (int k = 1; k < v.splits; ++k) key = max(key, part[k]);
+        const bool ok = x == (long)(0xffffffffu - (uint32_t)key);
         prob = ok ? 1.f : 0.f;
+        if (!ok) atomicMin(&s.first, i);
       } else {
         double p = 0.0, q = v.draft ? 0.0 : 1.0;
         if (x >= 0 && x < v.V) {
-          p = weight(to_float(target_row<T>(v, b, i).p[x]), st[2 * i], v.inv_temperature) / st[2 * i + 1];
-          const double* sd = st + 2 * (v.drafts + 1 + i);
-          if (v.draft) q = weight(to_float(draft_row<T>(v, b, i).p[x]), sd[0], v.inv_temperature) / sd[1];
+          const double2 sp = row_sum(i);
+          p = exp2_64th(((double)to_float(target_row<T>(v, b, i).p[x]) - sp.x) * scale, s.table) / sp.y;
+          if (v.draft) {
+            const double2 sq = row_sum(n + 1 + i);
+            q = exp2_64th(((double)to_float(draft_row<T>(v, b, i).p[x]) - sq.x) * scale, s.table) / sq.y;
+          }
         }
-        ok = uniform(v, b, i) * q < p;
+        const double uq = uniform(v, b, i) * q;
         prob = p > 0.0 ? (p >= q ? 1.f : (float)(p / q)) : p == 0.0 ? 0.f : NAN;
+        // the sums may be off by 2^-15 each: `first_sure` is rejected whatever they are, `first` might be
+        if (!(uq * (1.0 + 0x1p-13) < p)) atomicMin(&s.first, i);
+        if (!(uq < p * (1.0 + 0x1p-13)) || p == 0.0) atomicMin(&s.first_sure, i);
       }
-      if (!ok) atomicMin(first, i);
     }
-    v.accept_prob[(long)b * v.drafts + i] = prob;
+    if (rank == 0) v.accept_prob[(long)b * n + i] = prob;
   }
   __syncthreads();
-  const int a = *first;
-  for (int i = threadIdx.x; i <= v.drafts; i += kVerifyThreads)
-    if (i != a) v.tokens[(long)b * (v.drafts + 1) + i] = i < a ? v.draft_ids[(long)b * v.drafts + i] : -1;
-  if (threadIdx.x == 0) v.accepted[b] = a;
-  return a;
-}
-
-// ----------------------------------------------------------------------------
-// Sequences: acceptance, then the next token.  One CTA per sequence; every thread draws from one run of vectors.
-// ----------------------------------------------------------------------------
-template <typename T>
-__global__ void __launch_bounds__(kVerifyThreads) verify_draw_kernel(Verify v) {
-  grid_dependency_sync();
-  __shared__ int first;
-  __shared__ double part[kVerifyThreads];
-  __shared__ int chosen, last;
-  const int b = blockIdx.x, len = draft_len(v, b), tid = threadIdx.x;
-  const int a = accept<T>(v, b, len, &first);
-  const double* st = v.stats + (long)b * (2 * v.drafts + 1) * 2;
-  long* token = v.tokens + (long)b * (v.drafts + 1) + a;
+  int a = s.first;
+  if (v.sampled) {
+    // drafts whose acceptance hangs on the sums' errors, up to the first that is rejected
+    const int sure = s.first_sure;
+    for (; a < sure; ++a) {
+      const double2 sp = row_sum(a), sq = v.draft ? row_sum(n + 1 + a) : make_double2(0.0, 1.0);
+      const long x = v.draft_ids[(long)b * n + a];          // in the vocabulary: p(x) > 0
+      const double ep = exp2_64th(((double)to_float(target_row<T>(v, b, a).p[x]) - sp.x) * scale, s.table);
+      const double eq = v.draft ? exp2_64th(((double)to_float(draft_row<T>(v, b, a).p[x]) - sq.x) * scale, s.table) : 1.0;
+      const double u = uniform(v, b, a);
+      if (u * (eq / sq.y) * (1.0 + 0x1p-13) < ep / sp.y) continue;       // far enough from the border
+      const double2 sums = exact_sums(a, v.draft != nullptr, sp.x, sq.x);
+      if (!(u * (v.draft ? eq / sums.y : 1.0) < ep / sums.x)) break;
+    }
+  }
+  long* token = v.tokens + at + a;
+  if (rank == 0) {
+    for (int i = tid; i <= n; i += kDrawThreads)
+      if (i != a) v.tokens[at + i] = i < a ? v.draft_ids[(long)b * n + i] : -1;
+    if (tid == 0) v.accepted[b] = a;
+  }
   if (!v.sampled) {
-    if (tid == 0) *token = (long)st[2 * a];
+    if (rank == 0 && tid == 0) {
+      const unsigned long long* part = v.parts + ((long)b * v.rows + a) * v.splits;
+      unsigned long long key = part[0];
+      for (int k = 1; k < v.splits; ++k) key = max(key, part[k]);
+      *token = (long)(0xffffffffu - (uint32_t)key);
+    }
     return;
   }
-  const Row<T> p = target_row<T>(v, b, a);
-  const bool rejected = a < len;
-  const long x = rejected ? v.draft_ids[(long)b * v.drafts + a] : -1;
-  const double* sp = st + 2 * a;
-  const double* sq = st + 2 * (v.drafts + 1 + a);
-  const T* q = rejected && v.draft ? draft_row<T>(v, b, a).p : nullptr;
-  const double top_p = sp[0], sum_p = sp[1], top_q = q ? sq[0] : 0.0, sum_q = q ? sq[1] : 1.0;
-  const int nv = p.vectors(), per = (nv + kVerifyThreads - 1) / kVerifyThreads;
-  bool rest = rejected;                      // weights are max(p - q, 0); false: p
-  auto weigh = [&](int c, float xp) {
-    const double w = weight(xp, top_p, v.inv_temperature) / sum_p;
-    if (!rest) return w;
-    if (q == nullptr) return c == x ? 0.0 : w;
-    const double d = w - weight(to_float(q[c]), top_q, v.inv_temperature) / sum_q;
-    return d > 0.0 ? d : 0.0;
-  };
-  double total;
-  for (;;) {
-    double s = 0.0;
-    for (int i = tid * per; i < min((tid + 1) * per, nv); ++i) {
-      float e[Row<T>::kVec];
-      RowVec<T>::unpack(p.load(i), e);
-      const int c = p.column(i);
-#pragma unroll
-      for (int j = 0; j < Row<T>::kVec; ++j)
-        if (c + j >= 0 && c + j < v.V) s += weigh(c + j, e[j]);
+
+  // ---- the next token
+  Weigher<T> w = {target_row<T>(v, b, a), nullptr, s.table, scale, 0.0, 0.0, 1.0, 1.0, -1, kPlain};
+  const double m_p = row_sum(a).x;
+  w.less_p = m_p * scale;
+  if (a < len) {
+    w.kind = kWithout;
+    w.x = v.draft_ids[(long)b * n + a];
+    if (v.draft) {
+      const double m_q = row_sum(n + 1 + a).x;
+      const double2 sums = exact_sums(a, true, m_p, m_q);
+      w.kind = kRest;
+      w.q = draft_row<T>(v, b, a).p;
+      w.less_q = m_q * scale;
+      w.by_p = 1.0 / sums.x;
+      w.by_q = 1.0 / sums.y;
     }
-    __syncthreads();
-    part[tid] = s;
-    __syncthreads();
-    if (tid == 0) {
-      for (int i = 1; i < kVerifyThreads; ++i) part[i] += part[i - 1];
-      chosen = v.V;
-      last = -1;
-    }
-    __syncthreads();
-    total = part[kVerifyThreads - 1];
-    if (total > 0.0 || !rest) break;
-    rest = false;
   }
-  const double goal = uniform(v, b, v.drafts) * total;
-  const double before = tid ? part[tid - 1] : 0.0;
-  double s = 0.0;
-  int mine = v.V, end = -1;
-  if (part[tid] > before)
-    for (int i = tid * per; i < min((tid + 1) * per, nv); ++i) {
-      float e[Row<T>::kVec];
-      RowVec<T>::unpack(p.load(i), e);
-      const int c = p.column(i);
-#pragma unroll
-      for (int j = 0; j < Row<T>::kVec; ++j) {
-        if (c + j < 0 || c + j >= v.V) continue;
-        const double w = weigh(c + j, e[j]);
-        s += w;
-        if (w > 0.0) end = c + j;
-        if (w > 0.0 && before + s > goal && mine == v.V) mine = c + j;
-      }
+  // a warp weighs a run of neighbouring vectors
+  const int2 run = run_of(w.p);
+  const int share = (run.y - run.x + kDrawWarps - 1) / kDrawWarps;
+  auto warp_run = [&](int k) { return make_int2(min(run.x + k * share, run.y), min(run.x + (k + 1) * share, run.y)); };
+  double rest = 0.0;                               // weight up to the token, from this CTA's first vector on
+  int owner = -1;
+  for (;;) {
+    const int2 mine = warp_run(warp);
+    const double part = block_sum(w.sum_run(mine.x + lane, mine.y, 32));
+    const double total = cluster_total(make_double2(part, 0.0)).x;
+    if (!(total > 0.0)) {
+      if (w.kind == kPlain) break;
+      w.kind = kPlain;                              // no mass but the draft's: from the target itself
+      continue;
     }
-  atomicMin(&chosen, mine);
-  atomicMax(&last, end);
-  __syncthreads();
-  // by rounding the goal may lie behind the last sum; no id has any weight if the target's row is not a distribution
-  if (tid == 0) *token = chosen < v.V ? chosen : last;
+    // the first CTA whose weights pass the goal; by rounding the goal may lie behind all: the last one with any weight
+    const double goal = uniform(v, b, n) * total;
+    double up_to = 0.0;
+    for (int k = 0; k < C && !(owner >= 0 && up_to > goal); ++k) {
+      const double x = reinterpret_cast<const double2*>(&s.cta_part[turn ^ 1][k])->x;
+      if (!(x > 0.0)) continue;
+      owner = k;
+      rest = goal - up_to;
+      up_to += x;
+    }
+    break;
+  }
+  if (owner < 0 && rank == 0 && tid == 0) *token = -1;      // the target's row is no distribution
+  if (owner != rank) return;
+  // the same among the runs of this CTA's warps, and among eight parts of the one that it is
+  auto pick = [&](int2 whole, int part) {
+    int k = -1;
+    double up_to = 0.0, from = 0.0;
+    for (int q = 0; q < kDrawWarps && !(k >= 0 && up_to > rest); ++q) {
+      const double x = s.warp_total[q];
+      if (!(x > 0.0)) continue;
+      k = q;
+      from = up_to;
+      up_to += x;
+    }
+    rest -= from;
+    k = max(k, 0);
+    return make_int2(min(whole.x + k * part, whole.y), min(whole.x + (k + 1) * part, whole.y));
+  };
+  const int2 coarse = pick(run, share);
+  const int finer = (coarse.y - coarse.x + kDrawWarps - 1) / kDrawWarps;
+  const int from = min(coarse.x + warp * finer, coarse.y), to = min(from + finer, coarse.y);
+  (void)block_sum(w.sum_run(from + lane, to, 32));
+  const int2 fine = pick(coarse, finer);
+  if (warp != 0) return;
+  for (int i0 = fine.x; i0 < fine.y; i0 += 32) {
+    double x = w.sum_run(i0 + lane, min(fine.y, i0 + lane + 1), 1), up_to = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, up_to, o);
+      if (lane >= o) up_to += y;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, up_to > rest && x > 0.0);
+    if (past) {
+      if (lane != __ffs(past) - 1) return;
+      double sum = up_to - x;
+      int chosen = -1;
+      for (int j = 0; j < Row<T>::kVec && !(chosen >= 0 && sum > rest); ++j) {
+        const int col = w.p.column(i0 + lane) + j;
+        const double y = col >= 0 && col < v.V ? w.of(w.p.p[col], col) : 0.0;
+        if (!(y > 0.0)) continue;
+        chosen = col;
+        sum += y;
+      }
+      *token = chosen;
+      return;
+    }
+    rest -= __shfl_sync(0xffffffffu, up_to, 31);
+  }
+  // by rounding the goal lies behind this part: its last column with any weight
+  if (lane == 0) {
+    int col = min(w.p.column(fine.y), v.V) - 1;
+    const int least = max(w.p.column(fine.x), 0);
+    while (col > least && !(w.of(w.p.p[col], col) > 0.0)) --col;
+    *token = col;
+  }
+}
+
+// Parts of a row: enough CTAs for eight an SM, as long as each thread has kRowAhead vectors.
+int splits_of(long rows, int V, int is_f32) {
+  const long most = V / (is_f32 ? 4 : 8) / (kRowAhead * kRowThreads), want = (8L * mmt_sm_count() + rows - 1) / (rows > 0 ? rows : 1);
+  const long n = want < most ? want : most;
+  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 
 template <typename T>
 int launch_verify(const Verify& v, void* stream) {
-  const int rows = v.sampled && v.draft ? 2 * v.drafts + 1 : v.drafts + 1;
-  const int e = (int)launch_dependent(verify_rows_kernel<T>, dim3(rows, v.batch), kVerifyThreads, 0, VR_STREAM(stream), v);
+  const dim3 grid(v.splits, v.rows, v.batch);
+  const int e = (int)(v.sampled ? launch_dependent(verify_rows_kernel<T, true>, grid, kRowThreads, 0, VR_STREAM(stream), v)
+                                : launch_dependent(verify_rows_kernel<T, false>, grid, kRowThreads, 0, VR_STREAM(stream), v));
   if (e) return e;
-  return (int)launch_dependent(verify_draw_kernel<T>, v.batch, kVerifyThreads, 0, VR_STREAM(stream), v);
+  const unsigned C = v.sampled ? kDrawCluster : 1;
+  return (int)launch_cluster(verify_draw_kernel<T>, v.batch * C, kDrawThreads, C, 0, VR_STREAM(stream), v);
 }
 
 }  // namespace
@@ -246,10 +530,13 @@ int launch_verify(const Verify& v, void* stream) {
 extern "C" {
 
 int mmt_verify_bytes() { return (int)sizeof(Verify); }
+// Parts that `rows` rows of V columns are read in.
+int mmt_verify_splits(long rows, int V, int is_f32) { return splits_of(rows, V, is_f32); }
 
 int mmt_verify_drafts(const void* words, void* stream) {
   const Verify& v = *reinterpret_cast<const Verify*>(words);
-  if (v.batch < 0 || v.batch > 65535 || v.drafts < 0 || v.drafts > 65535 || v.V < 1) return -2;
+  if (v.batch < 0 || v.batch > 65535 || v.drafts < 0 || v.rows > 65535 || v.rows < v.drafts + 1 || v.V < 1 || v.splits < 1)
+    return -2;
   if (v.batch == 0) return 0;
   return v.is_f32 ? launch_verify<float>(v, stream) : launch_verify<bf16>(v, stream);
 }

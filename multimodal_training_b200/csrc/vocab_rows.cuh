@@ -102,6 +102,118 @@ struct Row {
   }
 };
 
+// ----------------------------------------------------------------------------
+// Small arithmetic
+// ----------------------------------------------------------------------------
+MMT_DEVICE float pow2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+MMT_DEVICE float thread_max(const uint4& u, float m, bf16) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  __nv_bfloat162 t = *reinterpret_cast<const __nv_bfloat162*>(&w[0]);
+#pragma unroll
+  for (int j = 1; j < 4; ++j) t = __hmax2(t, *reinterpret_cast<const __nv_bfloat162*>(&w[j]));
+  return fmaxf(m, fmaxf(__low2float(t), __high2float(t)));
+}
+MMT_DEVICE float thread_max(const uint4& u, float m, float) {
+  return fmaxf(fmaxf(m, fmaxf(__uint_as_float(u.x), __uint_as_float(u.y))),
+               fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+}
+// Largest of a warp's values, NaN left out.
+MMT_DEVICE float warp_top(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+// Two fp32 values in one 64-bit register: an instruction works on both.
+typedef unsigned long long f32x2;
+MMT_DEVICE f32x2 both(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+MMT_DEVICE float2 apart(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+MMT_DEVICE f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+MMT_DEVICE f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+MMT_DEVICE f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Order-preserving bits of a logit; kBits of them.
+template <typename T>
+struct Key;
+template <>
+struct Key<bf16> {
+  static constexpr int kBits = 16;
+  static MMT_DEVICE uint32_t of(bf16 x) {
+    uint32_t b = __bfloat16_as_ushort(x);
+    if ((b & 0x7fffu) > 0x7f80u) return 0xffffu;
+    if (b == 0x8000u) b = 0;
+    return b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
+  }
+  // The logit of a key, if the key tells.
+  static MMT_DEVICE bool back(uint32_t key, bf16& x) {
+    x = __ushort_as_bfloat16((unsigned short)(key & 0x8000u ? key & 0x7fffu : ~key));
+    return key != 0x8000u && key != 0xffffu;
+  }
+  // The largest of a vector's keys, and the upper 16 bits of it.
+  static MMT_DEVICE uint32_t top(const uint4& u) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    __nv_bfloat162 t = *reinterpret_cast<const __nv_bfloat162*>(&w[0]);
+#pragma unroll
+    for (int j = 1; j < 4; ++j) t = __hmax2_nan(t, *reinterpret_cast<const __nv_bfloat162*>(&w[j]));
+    return of(__hmax_nan(__low2bfloat16(t), __high2bfloat16(t)));
+  }
+  static MMT_DEVICE uint32_t top16(const uint4& u) { return top(u); }
+};
+template <>
+struct Key<float> {
+  static constexpr int kBits = 32;
+  static MMT_DEVICE uint32_t of(float x) {
+    uint32_t b = __float_as_uint(x);
+    if ((b & 0x7fffffffu) > 0x7f800000u) return 0xfffffffeu;          // one below the largest: there is a key above it
+    if (b == 0x80000000u) b = 0;
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+  }
+  static MMT_DEVICE bool back(uint32_t key, float& x) {
+    x = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+    return key != 0x80000000u && key != 0xfffffffeu;
+  }
+  static MMT_DEVICE uint32_t top(const uint4& u) {
+    return max(max(of(__uint_as_float(u.x)), of(__uint_as_float(u.y))), max(of(__uint_as_float(u.z)), of(__uint_as_float(u.w))));
+  }
+  static MMT_DEVICE uint32_t top16(const uint4& u) { return top(u) >> 16; }
+};
+
+// Element j (of as many as a vector has) of a vector.
+template <typename T>
+MMT_DEVICE T element(const uint4& v, int j);
+template <>
+MMT_DEVICE bf16 element<bf16>(const uint4& v, int j) {
+  const uint32_t w = j & 4 ? (j & 2 ? v.w : v.z) : (j & 2 ? v.y : v.x);
+  return __ushort_as_bfloat16((unsigned short)(j & 1 ? w >> 16 : w));
+}
+template <>
+MMT_DEVICE float element<float>(const uint4& v, int j) {
+  return __uint_as_float(j & 2 ? (j & 1 ? v.w : v.z) : (j & 1 ? v.y : v.x));
+}
+
 // Sum / maximum over a block of kThreads; `red` holds kThreads / 32 values and may be used again at once.
 template <int kThreads, typename F>
 MMT_DEVICE F block_total(F v, F* red) {
@@ -143,6 +255,13 @@ MMT_DEVICE uint32_t cluster_size() {
 // All threads of all CTAs of the cluster; shared-memory writes in front of it are seen behind it, in every CTA.
 MMT_DEVICE void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Writes to the place in CTA `rank`'s shared memory that `p` has in this CTA's.
+MMT_DEVICE void cluster_store(float4* p, uint32_t rank, float4 v) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+               : "memory");
 }
 // Writes to the place in CTA `rank`'s shared memory that `p` has in this CTA's, and counts the 16 bytes into the mbarrier
 // there that `bar` is here.

@@ -531,12 +531,13 @@ class _VerifyWords(ctypes.Structure):
                 ("target_row", ctypes.c_long), ("draft_seq", ctypes.c_long), ("draft_row", ctypes.c_long),
                 ("draft_ids", ctypes.c_void_p), ("uniforms", ctypes.c_void_p), ("lens", ctypes.c_void_p),
                 ("accepted", ctypes.c_void_p), ("tokens", ctypes.c_void_p), ("accept_prob", ctypes.c_void_p),
-                ("stats", ctypes.c_void_p), ("inv_temperature", ctypes.c_double), ("batch", ctypes.c_int),
+                ("parts", ctypes.c_void_p), ("inv_temperature", ctypes.c_double), ("batch", ctypes.c_int),
                 ("drafts", ctypes.c_int), ("V", ctypes.c_int), ("is_f32", ctypes.c_int), ("uniforms_f64", ctypes.c_int),
-                ("sampled", ctypes.c_int)]
+                ("sampled", ctypes.c_int), ("rows", ctypes.c_int), ("splits", ctypes.c_int)]
 
 
 nv.declare("mmt_verify_bytes", nv.c_int, [])
+nv.declare("mmt_verify_splits", nv.c_int, [nv.c_long, nv.c_int, nv.c_int])
 nv.declare("mmt_verify_drafts", nv.c_int, [nv._P, nv._P])
 
 
@@ -648,8 +649,8 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
         _integral(draft_lens, "draft_lens")
         if draft_lens.shape != (B,):
             raise ValueError(f"draft_lens {tuple(draft_lens.shape)} must be ({B},)")
-    if B > 65535 or n > 65535:
-        raise ValueError(f"at most 65535 sequences and drafts, got {B} and {n}")
+    if B > 65535 or n > 32767:
+        raise ValueError(f"at most 65535 sequences and 32767 drafts, got {B} and {n}")
     gpu = _on_gpu(target_logits, draft_ids, draft_logits, uniforms, draft_lens)
     draft_ids = _ids64(draft_ids).contiguous()
     lens = None if draft_lens is None else _ids64(draft_lens).contiguous()
@@ -668,15 +669,17 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
     accepted = torch.empty(B, device=dev, dtype=torch.int64)
     tokens = torch.empty(B, n + 1, device=dev, dtype=torch.int64)
     prob = torch.empty(B, n, device=dev, dtype=torch.float32)
-    stats = torch.empty(B, 2 * n + 1, 2, device=dev, dtype=torch.float64)
     if B:
+        rows, is_f32 = n + 1 + (n if draft is not None else 0), int(target.dtype == torch.float32)
+        splits = nv.lib().mmt_verify_splits(B * rows, V, is_f32)
+        parts = torch.empty(B * rows * splits, device=dev, dtype=torch.int64)
         w = _VerifyWords(target=target.data_ptr(), draft=nv.ptr(draft), target_seq=target.stride(0),
                          target_row=target.stride(1), draft_seq=draft.stride(0) if draft is not None else 0,
                          draft_row=draft.stride(1) if draft is not None else 0, draft_ids=draft_ids.data_ptr(),
                          uniforms=nv.ptr(uniforms), lens=nv.ptr(lens), accepted=accepted.data_ptr(),
-                         tokens=tokens.data_ptr(), accept_prob=prob.data_ptr(), stats=stats.data_ptr(),
+                         tokens=tokens.data_ptr(), accept_prob=prob.data_ptr(), parts=parts.data_ptr(),
                          inv_temperature=1.0 / temperature if temperature else 0.0, batch=B, drafts=n, V=V,
-                         is_f32=int(target.dtype == torch.float32),
+                         is_f32=is_f32, rows=rows, splits=splits,
                          uniforms_f64=int(uniforms is not None and uniforms.dtype == torch.float64),
                          sampled=int(temperature > 0.0))
         nv.call("mmt_verify_drafts", ctypes.addressof(w), nv.stream())
