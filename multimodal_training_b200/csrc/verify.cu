@@ -182,11 +182,14 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(Verify v) {
 // ----------------------------------------------------------------------------
 // Sequences.  The first CTA of a sequence's cluster writes its answers.
 // ----------------------------------------------------------------------------
+constexpr int kChunk = 32;            // drafts that are looked at together
+enum Verdict { kStands, kHangs, kFalls };
 struct DrawShared {
   double table[64];                   // 2^(i / 64)
   double warp_total[kDrawWarps];
   float4 cta_part[2][kDrawCluster];   // two doubles each
-  int first, first_sure;
+  int verdict[kChunk];                // of a chunk of drafts: stands, hangs on the sums' errors, falls
+  double2 logits[kChunk], less[kChunk];       // for those that hang: weights of the draft, largest logits
 };
 
 // 2^(z / 64) in fp64 from a table and a polynomial (Tang, Table-driven implementation of the exponential function, 1989):
@@ -277,26 +280,31 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(Verify v) {
   const int b = blockIdx.x / C, n = v.drafts, len = draft_len(v, b);
   const long at = (long)b * (n + 1);
   if (tid < 64) s.table[tid] = exp2((double)tid / 64.0);
-  if (tid == 0) s.first = s.first_sure = len;
-  __syncthreads();
   cluster_barrier();                               // every CTA has started: its shared memory may be written
   int turn = 0;
   const double scale = 64.0 * kLog2e * v.inv_temperature;
 
-  // largest logit and normaliser of a row, from its parts
+  // largest logit and normaliser of a row, from its parts; by a warp
   const float c = scale_of(v);
   auto row_sum = [&](int r) {
     const float2* part = reinterpret_cast<const float2*>(v.parts + ((long)b * v.rows + r) * v.splits);
-    float m = part[0].x;
-    for (int k = 1; k < v.splits; ++k) m = fmaxf(m, part[k].x);
-    double sum = 0.0;
-    for (int k = 0; k < v.splits; ++k) {
-      const float2 a = part[k];
-      // the part's sum is relative to fl(its largest c)
-      const double by = a.x == -INFINITY ? 1.0 : exp2((double)__fmul_rn(a.x, c) - (double)m * (double)c);
-      sum += (double)a.y * by;
-    }
-    return make_double2((double)m, sum);
+    const float2 none = make_float2(-INFINITY, 0.f);
+    const float2 x = lane < v.splits ? part[lane] : none, y = lane + 32 < v.splits ? part[lane + 32] : none;
+    const float m = warp_top(fmaxf(x.x, y.x));
+    // a part's sum is relative to fl(its largest c)
+    auto of = [&](float2 p) {
+      const double less = (double)__fmul_rn(p.x, c) - (double)m * (double)c;
+      return p.x == -INFINITY ? (double)p.y : (double)p.y * exp2_64th(64.0 * less, s.table);
+    };
+    return make_double2((double)m, warp_total_of(of(x) + of(y)));
+  };
+  // largest logit's id of a row without sampling; by a warp
+  auto row_choice = [&](int r) {
+    const unsigned long long* part = v.parts + ((long)b * v.rows + r) * v.splits;
+    unsigned long long key = max(lane < v.splits ? part[lane] : 0ull, lane + 32 < v.splits ? part[lane + 32] : 0ull);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+    return (long)(0xffffffffu - (uint32_t)key);
   };
   // a value of each CTA, summed in their order
   auto cluster_total = [&](double2 mine) {
@@ -346,65 +354,60 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(Verify v) {
   };
 
   // ---- acceptance: every CTA decides for itself
-  for (int i = tid; i < n; i += kDrawThreads) {
-    float prob = 0.f;
-    if (i < len) {
+  int a = len;
+  for (int c0 = 0; c0 < len; c0 += kChunk) {
+    const int in_chunk = min(kChunk, len - c0);
+    for (int j = warp; j < in_chunk; j += kDrawWarps) {
+      const int i = c0 + j;
       const long x = v.draft_ids[(long)b * n + i];
+      float prob;
+      int verdict;
       if (!v.sampled) {
-        const unsigned long long* part = v.parts + ((long)b * v.rows + i) * v.splits;
-        unsigned long long key = part[0];
-        for (int k = 1; k < v.splits; ++k) key = max(key, part[k]);
-        const bool ok = x == (long)(0xffffffffu - (uint32_t)key);
-        prob = ok ? 1.f : 0.f;
-        if (!ok) atomicMin(&s.first, i);
+        verdict = x == row_choice(i) ? kStands : kFalls;
+        prob = verdict == kStands ? 1.f : 0.f;
       } else {
-        double p = 0.0, q = v.draft ? 0.0 : 1.0;
-        if (x >= 0 && x < v.V) {
-          const double2 sp = row_sum(i);
-          p = exp2_64th(((double)to_float(target_row<T>(v, b, i).p[x]) - sp.x) * scale, s.table) / sp.y;
-          if (v.draft) {
-            const double2 sq = row_sum(n + 1 + i);
-            q = exp2_64th(((double)to_float(draft_row<T>(v, b, i).p[x]) - sq.x) * scale, s.table) / sq.y;
-          }
+        const bool known = x >= 0 && x < v.V;
+        const double2 sp = row_sum(i), sq = v.draft ? row_sum(n + 1 + i) : make_double2(0.0, 1.0);
+        double ep = 0.0, eq = v.draft ? 0.0 : 1.0;
+        if (known) {
+          ep = exp2_64th(((double)to_float(target_row<T>(v, b, i).p[x]) - sp.x) * scale, s.table);
+          if (v.draft) eq = exp2_64th(((double)to_float(draft_row<T>(v, b, i).p[x]) - sq.x) * scale, s.table);
         }
-        const double uq = uniform(v, b, i) * q;
+        const double p = known ? ep / sp.y : 0.0, q = v.draft && !known ? 0.0 : eq / sq.y, uq = uniform(v, b, i) * q;
         prob = p > 0.0 ? (p >= q ? 1.f : (float)(p / q)) : p == 0.0 ? 0.f : NAN;
-        // the sums may be off by 2^-15 each: `first_sure` is rejected whatever they are, `first` might be
-        if (!(uq * (1.0 + 0x1p-13) < p)) atomicMin(&s.first, i);
-        if (!(uq < p * (1.0 + 0x1p-13)) || p == 0.0) atomicMin(&s.first_sure, i);
+        // both sums may be off by 2^-15
+        verdict = uq * (1.0 + 0x1p-13) < p ? kStands : uq < p * (1.0 + 0x1p-13) && p > 0.0 ? kHangs : kFalls;
+        if (lane == 0) {
+          s.logits[j] = make_double2(ep, eq);
+          s.less[j] = make_double2(sp.x, sq.x);
+        }
+      }
+      if (lane == 0) {
+        s.verdict[j] = verdict;
+        if (rank == 0) v.accept_prob[(long)b * n + i] = prob;
       }
     }
-    if (rank == 0) v.accept_prob[(long)b * n + i] = prob;
-  }
-  __syncthreads();
-  int a = s.first;
-  if (v.sampled) {
-    // drafts whose acceptance hangs on the sums' errors, up to the first that is rejected
-    const int sure = s.first_sure;
-    for (; a < sure; ++a) {
-      const double2 sp = row_sum(a), sq = v.draft ? row_sum(n + 1 + a) : make_double2(0.0, 1.0);
-      const long x = v.draft_ids[(long)b * n + a];          // in the vocabulary: p(x) > 0
-      const double ep = exp2_64th(((double)to_float(target_row<T>(v, b, a).p[x]) - sp.x) * scale, s.table);
-      const double eq = v.draft ? exp2_64th(((double)to_float(draft_row<T>(v, b, a).p[x]) - sq.x) * scale, s.table) : 1.0;
-      const double u = uniform(v, b, a);
-      if (u * (eq / sq.y) * (1.0 + 0x1p-13) < ep / sp.y) continue;       // far enough from the border
-      const double2 sums = exact_sums(a, v.draft != nullptr, sp.x, sq.x);
-      if (!(u * (v.draft ? eq / sums.y : 1.0) < ep / sums.x)) break;
+    __syncthreads();
+    for (int j = 0; j < in_chunk && a == len; ++j) {
+      bool falls = s.verdict[j] == kFalls;
+      if (s.verdict[j] == kHangs) {
+        const double2 e = s.logits[j], sums = exact_sums(c0 + j, v.draft != nullptr, s.less[j].x, s.less[j].y);
+        falls = !(uniform(v, b, c0 + j) * (v.draft ? e.y / sums.y : 1.0) < e.x / sums.x);
+      }
+      if (falls) a = c0 + j;
     }
+    __syncthreads();
   }
-  long* token = v.tokens + at + a;
   if (rank == 0) {
+    for (int i = len + tid; i < n; i += kDrawThreads) v.accept_prob[(long)b * n + i] = 0.f;
     for (int i = tid; i <= n; i += kDrawThreads)
       if (i != a) v.tokens[at + i] = i < a ? v.draft_ids[(long)b * n + i] : -1;
     if (tid == 0) v.accepted[b] = a;
   }
+  long* token = v.tokens + at + a;
   if (!v.sampled) {
-    if (rank == 0 && tid == 0) {
-      const unsigned long long* part = v.parts + ((long)b * v.rows + a) * v.splits;
-      unsigned long long key = part[0];
-      for (int k = 1; k < v.splits; ++k) key = max(key, part[k]);
-      *token = (long)(0xffffffffu - (uint32_t)key);
-    }
+    const long choice = row_choice(a);
+    if (rank == 0 && tid == 0) *token = choice;
     return;
   }
 
