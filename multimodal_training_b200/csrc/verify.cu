@@ -17,9 +17,9 @@ namespace {
 
 constexpr int kRowThreads = 256;                  // of a CTA that reads a part of a row
 constexpr int kRowAhead = 4;                      // vectors that a thread loads before it works on them
-constexpr int kDrawThreads = 256;
+constexpr int kDrawThreads = 512;
 constexpr int kDrawWarps = kDrawThreads / 32;
-constexpr int kDrawCluster = 8;                   // CTAs that weigh a row
+constexpr int kDrawCluster = 16;                  // most CTAs that weigh a row
 constexpr double kLog2e = 1.44269504088896340736;
 
 struct Verify {
@@ -185,29 +185,35 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(Verify v) {
 constexpr int kChunk = 32;            // drafts that are looked at together
 enum Verdict { kStands, kHangs, kFalls };
 struct DrawShared {
-  double table[64];                   // 2^(i / 64)
+  double table[16];                   // 2^(i / 16)
   double warp_total[kDrawWarps];
   float4 cta_part[2][kDrawCluster];   // two doubles each
   int verdict[kChunk];                // of a chunk of drafts: stands, hangs on the sums' errors, falls
-  double2 logits[kChunk], less[kChunk];       // for those that hang: weights of the draft, largest logits
+  float2 logits[kChunk], largest[kChunk];     // of the draft, and of its rows (the target's, the draft model's)
 };
 
-// 2^(z / 64) in fp64 from a table and a polynomial (Tang, Table-driven implementation of the exponential function, 1989):
-// z = n + f with a whole n and |f| <= 1/2, 2^(n / 64) from the table and the exponent, 2^(f / 64) to 2^-54 by its series.
-MMT_DEVICE double exp2_64th(double z, const double* table) {
-  if (!(z > -64.0 * 1000.0)) return z == z ? 0.0 : z;
-  constexpr double kMagic = 6755399441055744.0;                  // 1.5 * 2^52: adding it rounds to a whole number
-  constexpr double kLn = 0.69314718055994530942 / 64.0;
-  const double shifted = z + kMagic, f = z - (shifted - kMagic);
-  const int n = __double2loint(shifted);
-  double p = fma(kLn * kLn * kLn * kLn * kLn / 120.0, f, kLn * kLn * kLn * kLn / 24.0);
-  p = fma(p, f, kLn * kLn * kLn / 6.0);
-  p = fma(p, f, kLn * kLn / 2.0);
-  p = fma(p, f, kLn);
-  p *= f;
-  const double t = table[n & 63], e = fma(t, p, t);
-  return __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
-}
+// 2^(x scale / 16 - whole / 16) in fp64, for a whole number `whole` near the largest x scale of the row: x scale - whole = n + f
+// with a whole n and |f| <= 1/2; 2^(n / 16) from a table of 16 (one word of each bank: no conflicts) and the exponent, 2^(f / 16)
+// by its series, whose rest is 2e-13 of it (Tang, Table-driven implementation of the exponential function, 1989).  Nine fp64
+// instructions and no branches: the drawn rows are bound by them.
+struct Powers16 {
+  static constexpr double kMagic = 6755399441055744.0;    // 1.5 * 2^52: a number near it is rounded to a whole one
+  double scale, shift;                            // shift = kMagic - whole
+  MMT_DEVICE Powers16(double scale_, double largest) : scale(scale_), shift(kMagic - rint(largest * scale_)) {}
+  MMT_DEVICE double of(float x, const double* table) const {
+    constexpr double L = 0.69314718055994530942 / 16.0, L2 = L * L;
+    const double shifted = fma((double)x, scale, shift), f = fma((double)x, scale, shift - shifted);
+    const int n = __double2loint(shifted);
+    double p = fma(L2 * L2 * L / 120.0, f, L2 * L2 / 24.0);
+    p = fma(p, f, L2 * L / 6.0);
+    p = fma(p, f, L2 / 2.0);
+    p = fma(p, f, L);
+    const double t = table[n & 15], e = fma(t, p * f, t);
+    const double power = __hiloint2double(__double2hiint(e) + ((n >> 4) << 20), __double2loint(e));
+    const double some = shifted > kMagic - 16000.0 ? power : 0.0;         // none below 2^-1000
+    return x == x ? some : (double)x;
+  }
+};
 
 // Weights of the columns of a row that a token is drawn from.
 enum Draw { kPlain, kWithout, kRest };            // p; p without one id; max(p - q, 0)
@@ -216,33 +222,36 @@ struct Weigher {
   Row<T> p;
   const T* q;
   const double* table;
-  double scale, less_p, less_q, by_p, by_q;       // exponents x scale - less in 64ths, times by
+  Powers16 of_p, of_q;
+  double by_p, by_q;
   long x;
   Draw kind;
+  MMT_DEVICE double rest(T xp, T xq) const {
+    const double d = of_p.of(to_float(xp), table) * by_p - of_q.of(to_float(xq), table) * by_q, r = d > 0.0 ? d : 0.0;
+    return d == d ? r : d;
+  }
   MMT_DEVICE double of(T xp, int c) const {
-    const double e = exp2_64th(fma((double)to_float(xp), scale, -less_p), table);
-    if (kind == kPlain) return e;
-    if (kind == kWithout) return c == x ? 0.0 : e;
-    const double d = e * by_p - exp2_64th(fma((double)to_float(q[c]), scale, -less_q), table) * by_q;
-    return d > 0.0 ? d : d == d ? 0.0 : d;
+    if (kind == kRest) return rest(xp, q[c]);
+    return kind == kWithout && c == x ? 0.0 : of_p.of(to_float(xp), table);
   }
   // Sum over vector i, whose logits are `u` if it is a whole one.
   MMT_DEVICE double sum(int i, const uint4& u) const {
     const int c = p.column(i);
     double s = 0.0;
     if (p.whole(i)) {
-      uint4 uq = u;
-      const bool pair = kind == kRest && Row<T>::lead_of(q) == p.lead;
-      if (pair) uq = *reinterpret_cast<const uint4*>(q + c);
+      if (kind == kRest && Row<T>::lead_of(q) == p.lead) {
+        const uint4 uq = *reinterpret_cast<const uint4*>(q + c);
 #pragma unroll
-      for (int j = 0; j < Row<T>::kVec; ++j) {
-        if (pair) {
-          const double d = exp2_64th(fma((double)to_float(element<T>(u, j)), scale, -less_p), table) * by_p -
-                           exp2_64th(fma((double)to_float(element<T>(uq, j)), scale, -less_q), table) * by_q;
-          s += d > 0.0 ? d : d == d ? 0.0 : d;
-        } else {
-          s += of(element<T>(u, j), c + j);
+        for (int j = 0; j < Row<T>::kVec; ++j) s += rest(element<T>(u, j), element<T>(uq, j));
+      } else if (kind != kRest) {
+#pragma unroll
+        for (int j = 0; j < Row<T>::kVec; ++j) {
+          const double e = of_p.of(to_float(element<T>(u, j)), table);
+          s += kind == kWithout && c + j == x ? 0.0 : e;
         }
+      } else {
+#pragma unroll 1
+        for (int j = 0; j < Row<T>::kVec; ++j) s += rest(element<T>(u, j), q[c + j]);
       }
     } else {
 #pragma unroll 1
@@ -272,17 +281,18 @@ MMT_DEVICE double warp_total_of(double v) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(Verify v) {
+__global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(Verify v) {
   grid_dependency_sync();
   __shared__ DrawShared s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int C = (int)cluster_size(), rank = (int)cluster_rank();
   const int b = blockIdx.x / C, n = v.drafts, len = draft_len(v, b);
   const long at = (long)b * (n + 1);
-  if (tid < 64) s.table[tid] = exp2((double)tid / 64.0);
+  if (tid < 16) s.table[tid] = exp2((double)tid / 16.0);
+  __syncthreads();
   cluster_barrier();                               // every CTA has started: its shared memory may be written
   int turn = 0;
-  const double scale = 64.0 * kLog2e * v.inv_temperature;
+  const double scale = 16.0 * kLog2e * v.inv_temperature;      // of Powers16
 
   // largest logit and normaliser of a row, from its parts; by a warp
   const float c = scale_of(v);
@@ -294,7 +304,7 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(Verify v) {
     // a part's sum is relative to fl(its largest c)
     auto of = [&](float2 p) {
       const double less = (double)__fmul_rn(p.x, c) - (double)m * (double)c;
-      return p.x == -INFINITY ? (double)p.y : (double)p.y * exp2_64th(64.0 * less, s.table);
+      return p.x == -INFINITY ? (double)p.y : (double)p.y * exp2(less);
     };
     return make_double2((double)m, warp_total_of(of(x) + of(y)));
   };
@@ -338,15 +348,15 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(Verify v) {
     const int nv = row.vectors(), per = (nv + C - 1) / C;
     return make_int2(min(rank * per, nv), min((rank + 1) * per, nv));
   };
-  // normalisers of a row of the target and of the draft model, in fp64
+  // normalisers of a row of the target and of the draft model, in fp64 (relative to the largest logits as Powers16 has them)
   auto exact_sums = [&](int i, bool with_q, double m_p, double m_q) {
-    Weigher<T> w = {target_row<T>(v, b, i), nullptr, s.table, scale, m_p * scale, 0.0, 1.0, 1.0, -1, kPlain};
+    Weigher<T> w = {target_row<T>(v, b, i), nullptr, s.table, Powers16(scale, m_p), Powers16(scale, m_p), 1.0, 1.0, -1, kPlain};
     int2 run = run_of(w.p);
     const double sum_p = block_sum(w.sum_run(run.x + tid, run.y, kDrawThreads));
     double sum_q = 0.0;
     if (with_q) {
       w.p = draft_row<T>(v, b, i);
-      w.less_p = m_q * scale;
+      w.of_p = Powers16(scale, m_q);
       run = run_of(w.p);
       sum_q = block_sum(w.sum_run(run.x + tid, run.y, kDrawThreads));
     }
@@ -368,18 +378,17 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(Verify v) {
       } else {
         const bool known = x >= 0 && x < v.V;
         const double2 sp = row_sum(i), sq = v.draft ? row_sum(n + 1 + i) : make_double2(0.0, 1.0);
-        double ep = 0.0, eq = v.draft ? 0.0 : 1.0;
-        if (known) {
-          ep = exp2_64th(((double)to_float(target_row<T>(v, b, i).p[x]) - sp.x) * scale, s.table);
-          if (v.draft) eq = exp2_64th(((double)to_float(draft_row<T>(v, b, i).p[x]) - sq.x) * scale, s.table);
-        }
-        const double p = known ? ep / sp.y : 0.0, q = v.draft && !known ? 0.0 : eq / sq.y, uq = uniform(v, b, i) * q;
+        const float xp = known ? to_float(target_row<T>(v, b, i).p[x]) : 0.f;
+        const float xq = known && v.draft ? to_float(draft_row<T>(v, b, i).p[x]) : 0.f;
+        auto share = [&](float x, double2 sum) { return exp2(((double)x - sum.x) * (scale / 16.0)) / sum.y; };
+        const double p = known ? share(xp, sp) : 0.0, q = !v.draft ? 1.0 : known ? share(xq, sq) : 0.0;
+        const double uq = uniform(v, b, i) * q;
         prob = p > 0.0 ? (p >= q ? 1.f : (float)(p / q)) : p == 0.0 ? 0.f : NAN;
         // both sums may be off by 2^-15
         verdict = uq * (1.0 + 0x1p-13) < p ? kStands : uq < p * (1.0 + 0x1p-13) && p > 0.0 ? kHangs : kFalls;
         if (lane == 0) {
-          s.logits[j] = make_double2(ep, eq);
-          s.less[j] = make_double2(sp.x, sq.x);
+          s.logits[j] = make_float2(xp, xq);
+          s.largest[j] = make_float2((float)sp.x, (float)sq.x);
         }
       }
       if (lane == 0) {
@@ -391,8 +400,10 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(Verify v) {
     for (int j = 0; j < in_chunk && a == len; ++j) {
       bool falls = s.verdict[j] == kFalls;
       if (s.verdict[j] == kHangs) {
-        const double2 e = s.logits[j], sums = exact_sums(c0 + j, v.draft != nullptr, s.less[j].x, s.less[j].y);
-        falls = !(uniform(v, b, c0 + j) * (v.draft ? e.y / sums.y : 1.0) < e.x / sums.x);
+        const float2 x = s.logits[j], m = s.largest[j];
+        const double2 sums = exact_sums(c0 + j, v.draft != nullptr, m.x, m.y);
+        const double q = v.draft ? Powers16(scale, m.y).of(x.y, s.table) / sums.y : 1.0;
+        falls = !(uniform(v, b, c0 + j) * q < Powers16(scale, m.x).of(x.x, s.table) / sums.x);
       }
       if (falls) a = c0 + j;
     }
@@ -412,9 +423,8 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(Verify v) {
   }
 
   // ---- the next token
-  Weigher<T> w = {target_row<T>(v, b, a), nullptr, s.table, scale, 0.0, 0.0, 1.0, 1.0, -1, kPlain};
   const double m_p = row_sum(a).x;
-  w.less_p = m_p * scale;
+  Weigher<T> w = {target_row<T>(v, b, a), nullptr, s.table, Powers16(scale, m_p), Powers16(scale, m_p), 1.0, 1.0, -1, kPlain};
   if (a < len) {
     w.kind = kWithout;
     w.x = v.draft_ids[(long)b * n + a];
@@ -423,7 +433,7 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(Verify v) {
       const double2 sums = exact_sums(a, true, m_p, m_q);
       w.kind = kRest;
       w.q = draft_row<T>(v, b, a).p;
-      w.less_q = m_q * scale;
+      w.of_q = Powers16(scale, m_q);
       w.by_p = 1.0 / sums.x;
       w.by_q = 1.0 / sums.y;
     }
@@ -457,7 +467,7 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw_kernel(Verify v) {
   }
   if (owner < 0 && rank == 0 && tid == 0) *token = -1;      // the target's row is no distribution
   if (owner != rank) return;
-  // the same among the runs of this CTA's warps, and among eight parts of the one that it is
+  // the same among the runs of this CTA's warps, and among as many parts of the one that it is
   auto pick = [&](int2 whole, int part) {
     int k = -1;
     double up_to = 0.0, from = 0.0;
@@ -524,8 +534,17 @@ int launch_verify(const Verify& v, void* stream) {
   const int e = (int)(v.sampled ? launch_dependent(verify_rows_kernel<T, true>, grid, kRowThreads, 0, VR_STREAM(stream), v)
                                 : launch_dependent(verify_rows_kernel<T, false>, grid, kRowThreads, 0, VR_STREAM(stream), v));
   if (e) return e;
-  const unsigned C = v.sampled ? kDrawCluster : 1;
-  return (int)launch_cluster(verify_draw_kernel<T>, v.batch * C, kDrawThreads, C, 0, VR_STREAM(stream), v);
+  auto kernel = verify_draw_kernel<T>;
+  static bool allowed = false;                     // clusters of more than eight
+  if (!allowed) {
+    const cudaError_t c = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (c != cudaSuccess) return (int)c;
+    allowed = true;
+  }
+  // two CTAs an SM
+  const int want = 2 * mmt_sm_count() / v.batch;
+  const unsigned C = !v.sampled || want < 1 ? 1 : want < kDrawCluster ? want : kDrawCluster;
+  return (int)launch_cluster(kernel, v.batch * C, kDrawThreads, C, 0, VR_STREAM(stream), v);
 }
 
 }  // namespace
