@@ -672,6 +672,25 @@ __global__ void __launch_bounds__(256) distill_scale_kernel(T* grad, long n, con
   if (e < n) from_float(to_float(grad[e]) * f, grad + e);
 }
 
+// out[r] = sum over the runs of parts[run][r], in their order, for the first min(*cnt, rows) rows of `cols` (a multiple of 8):
+// what mmt_gemm_bf16_split leaves.
+__global__ void __launch_bounds__(256) sum_runs_kernel(const float* parts, int runs, const int* cnt, int rows, int cols,
+                                                       bf16* __restrict__ out) {
+  grid_dependency_sync();
+  const long n8 = (long)min(max(*cnt, 0), rows) * cols / 8, stride = (long)rows * cols;
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < n8; i += gridDim.x * 256L) {
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    for (int r = 0; r < runs; ++r) {
+      const float4* p = reinterpret_cast<const float4*>(parts + r * stride + i * 8);
+      const float4 x = p[0], y = p[1];
+      a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+      b.x += y.x; b.y += y.y; b.z += y.z; b.w += y.w;
+    }
+    *reinterpret_cast<uint4*>(out + i * 8) =
+        make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
+  }
+}
+
 }  // namespace
 
 // The words of a call, in the order of ops/vocab_rows.py.
@@ -842,6 +861,15 @@ int mmt_distill_loss(const MmtDistill* d, float* loss, void* stream) {
   }
   return (int)launch_dependent(distill_loss_kernel, 1, kLossThreads, 0, VR_STREAM(stream), d->stats,
                                d->rows * (d->parts ? d->parts : 1), loss);
+}
+
+// The sum of the runs of a product whose K was cut (mmt_gemm_bf16_split), as [rows, cols] bf16.
+int mmt_sum_runs(const float* parts, int runs, const int* cnt, int rows, int cols, void* out, void* stream) {
+  if (cols % 8 || runs < 1) return -2;
+  if (rows == 0 || cols == 0) return 0;
+  const long want = ((long)rows * cols / 8 + 255) / 256, most = 8L * mmt_sm_count();
+  return (int)launch_dependent(sum_runs_kernel, (unsigned)(want < most ? want : most), 256, 0, VR_STREAM(stream), parts, runs,
+                               cnt, rows, cols, reinterpret_cast<bf16*>(out));
 }
 
 // n values at a 16-byte boundary.

@@ -83,6 +83,11 @@ struct GemmParams {
   float* sk_ws;
   int* sk_flags;
   int sk_epoch;
+  // --- K cut into k_split equal runs of k-blocks, for an output of few tiles and a long K: every run of a tile is a unit of
+  //     work of its own, whose fp32 result goes to its own array (C + run * split_stride floats); the caller adds them up.
+  //     Only with out_f32, without stream-K and collective roles.  1: off.
+  int k_split;
+  long split_stride;
   int dbg;                        // measurement only: bit 0 = operands are loaded once (ring filled, then reused), bit 1 = no
                                   // per-stage commit, bit 2 = no TMA stores, bit 3 = no epilogue work at all
   unsigned long long* clk;        // optional: CTA 0 writes {SM cycles, nanoseconds} it spent in the kernel
@@ -149,6 +154,7 @@ MMT_DEVICE void tile_coords(const GemmParams& p, int tile, int tiles_m, int bmt,
 //   kind 0: a whole tile;  kind 1: a run that stops before the tile's last k-block (partial sums go to the
 //   workspace);  kind 2: a run that ends the tile after other CTAs did its first k-blocks (their partial sums
 //   are added before the epilogue; `first_contrib` .. cta - 1 are those CTAs).
+// With k_split, k-blocks of run `first_contrib` of a tile, as kind 0.
 struct WorkItem {
   int tile, k0, k1, kind, first_contrib;
 };
@@ -156,6 +162,17 @@ struct WorkItem {
 // i-th work item of CTA `cta`: the stream-K runs first (partial sums before finishing runs, so that they are ready
 // when their tile ends), then this CTA's whole tiles.
 MMT_DEVICE bool work_item(const GemmParams& p, int i, int cta, int grid, int KB, int ntiles, WorkItem& w) {
+  if (p.k_split > 1) {
+    if (ntiles == 0) return false;
+    const int unit = cta + i * grid, run = unit / ntiles;
+    if (run >= p.k_split) return false;
+    w.tile = unit - run * ntiles;
+    w.k0 = (int)((long)KB * run / p.k_split);
+    w.k1 = (int)((long)KB * (run + 1) / p.k_split);
+    w.kind = 0;
+    w.first_contrib = run;
+    return true;
+  }
   const int i0 = i;
   const int full = ntiles - p.sk_tiles;
   int n_sk = 0;
@@ -319,7 +336,7 @@ MMT_DEVICE void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
 template <int BN>
 MMT_DEVICE void epilogue_block(const GemmParams& p, uint32_t tmem_acc, int row0, int col_tile0,
                                int q, int half, int lane, uint8_t* slab, uint32_t release_bar,
-                               const float* sk_part = nullptr, int sk_n = 0, long sk_stride = 0) {
+                               const float* sk_part = nullptr, int sk_n = 0, long sk_stride = 0, long c_offset = 0) {
   constexpr int kGroups = BN / 64;
   const bool tma_out = !p.out_f32 && p.tma_store;
   const int srow0 = row0 + q * 32;                 // first row of this warp's slab
@@ -399,7 +416,7 @@ MMT_DEVICE void epilogue_block(const GemmParams& p, uint32_t tmem_acc, int row0,
           }
         }
         if (p.out_f32) {
-          float* dst = reinterpret_cast<float*>(p.C) + grow * p.ldc + col;
+          float* dst = reinterpret_cast<float*>(p.C) + c_offset + grow * p.ldc + col;
           if (p.accumulate) {
             const float4 o0 = *reinterpret_cast<const float4*>(dst);
             const float4 o1 = *reinterpret_cast<const float4*>(dst + 4);
@@ -645,10 +662,10 @@ MMT_DEVICE void epilogue_fast(const GemmParams& p, const OutMaps& tmC, uint32_t 
 template <int BN>
 MMT_DEVICE void epilogue_any(const GemmParams& p, const OutMaps& tmC, bool remote, uint32_t tmem_acc, int row0,
                              int col_tile0, int q, int half, int lane, uint8_t* slab, uint32_t release_bar,
-                             const float* sk_part = nullptr, int sk_n = 0, long sk_stride = 0) {
+                             const float* sk_part = nullptr, int sk_n = 0, long sk_stride = 0, long c_offset = 0) {
   const bool fast = p.alpha == 1.0f && p.act == 0 && !p.accumulate && !p.out_f32 && sk_n == 0 && !(MMT_DBG & 12);
   if (!fast) {
-    epilogue_block<BN>(p, tmem_acc, row0, col_tile0, q, half, lane, slab, release_bar, sk_part, sk_n, sk_stride);
+    epilogue_block<BN>(p, tmem_acc, row0, col_tile0, q, half, lane, slab, release_bar, sk_part, sk_n, sk_stride, c_offset);
   } else if (p.bias) {
     if (p.residual) epilogue_fast<BN, true, true>(p, tmC, tmem_acc, row0, col_tile0, q, half, lane, slab, release_bar, remote);
     else epilogue_fast<BN, true, false>(p, tmC, tmem_acc, row0, col_tile0, q, half, lane, slab, release_bar, remote);
@@ -1060,7 +1077,7 @@ gemm_bf16_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         } else {
           epilogue_any<BN>(p, tmC, false, tmem_base + (uint32_t)(slot * BN), tm * BMT + h * BM, tn * BN, q, half, lane, slab,
                              smem_u32(&tempty[slot]), p.sk_ws + (long)w.first_contrib * kSlot + (long)h * BM * BN,
-                             n_contrib, kSlot);
+                             n_contrib, kSlot, p.k_split > 1 ? w.first_contrib * p.split_stride : 0);
         }
       }
       if (!ok) break;
@@ -1365,7 +1382,7 @@ int launch(const CUtensorMap& ta, const CUtensorMap& tb, const OutMaps& tc, cons
     if (e != cudaSuccess) return (int)e;
     attr_set = true;
   }
-  const int tiles = ((p.M + C_::BMT - 1) / C_::BMT) * ((p.N + BN - 1) / BN);
+  const int tiles = ((p.M + C_::BMT - 1) / C_::BMT) * ((p.N + BN - 1) / BN) * p.k_split;
   const int grid = (tiles < sms && p.sk_tiles == 0) ? tiles : sms;
   if (!p.local_only) {
     gemm_bf16_tcgen05<BN, MT><<<grid, kThreads, C_::SMEM, st>>>(ta, tb, tc, p);
@@ -1633,6 +1650,7 @@ struct GemmCount {
   int is_k, bucket;
   uint32_t mask;
   int mt, bn;
+  int split;                      // GemmParams::k_split, 0 or 1: off
 };
 
 // Model of the persistent kernel's time for a product without collective roles, in us, see choose_tile.
@@ -1843,6 +1861,8 @@ static int gemm_call(const void* A, const void* B, void* C, const void* bias, co
     if (p.rs_rows && (long)M > (long)p.rs_rows * p.rs_ranks) return -8;
   }
   // stream-K for a partial last wave (plain GEMMs on the 1-CTA kernels only)
+  p.k_split = count && count->split > 1 ? count->split : 1;
+  p.split_stride = (long)M * ldc;
   p.sk_tiles = 0;
   p.sk_ws = nullptr;
   p.sk_flags = nullptr;
@@ -1984,6 +2004,26 @@ extern "C" int mmt_gemm_bf16_counted(const void* A, const void* B, void* C, int 
     ++*launches;
   }
   return 0;
+}
+
+// Runs that K is cut into by mmt_gemm_bf16_split: as many as fill the SMs once with the output's 256-column tiles, each of 16
+// k-blocks or more; 1 where they are half full without.
+extern "C" int mmt_gemm_split(int M, int N, int K) {
+  const long tiles = (long)((M + 255) / 256) * ((N + 255) / 256), sms = mmt_sm_count(), kb = (K + BK - 1) / BK;
+  if (tiles < 1 || tiles * 2 > sms) return 1;
+  const long n = sms / tiles < kb / 16 ? sms / tiles : kb / 16;
+  return (int)(n < 1 ? 1 : n);
+}
+
+// Products of few rows over a long K: C[r] = A[:, run r of K] * B[run r of K], r < splits, each [M, N] fp32, over the first
+// min(max(*cnt, 0), M) rows (later rows are undefined).  A is [M][K], B is [K][N].  The gradient of 128 rows by a head of
+// 151936 x 2048 has eleven tiles and 2374 k-blocks: 752 us in whole tiles, with the same weight read by 144 CTAs 150.
+extern "C" int mmt_gemm_bf16_split(const void* A, const void* B, float* C, int M, int N, int K, int lda, int ldb,
+                                   const int* cnt, int splits, void* stream) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  GemmCount c = {cnt, 0, (M + 127) / 128 * 128, 1u, M > 128 ? 2 : 1, N > 192 ? 256 : N > 128 ? 192 : N > 64 ? 128 : 64, splits};
+  if (c.bn == 64) c.mt = 1;
+  return gemm_call(A, B, C, nullptr, nullptr, M, N, K, lda, ldb, N, 0, 0, 1, 0, 0, 1, 1.f, c.bn, &c, stream);
 }
 
 // Tuning knob: 1 = stream-K for partial last waves, 0 = whole tiles only (default).

@@ -162,6 +162,10 @@ nv.declare("mmt_distill_grad", nv.c_int, [nv._P, nv._P])
 nv.declare("mmt_distill_fused", nv.c_int, [nv._P, nv._P])
 nv.declare("mmt_distill_fused_columns", nv.c_long, [nv.c_int])
 nv.declare("mmt_distill_loss", nv.c_int, [nv._P, nv._P, nv._P])
+nv.declare("mmt_gemm_split", nv.c_int, [nv.c_int, nv.c_int, nv.c_int])
+nv.declare("mmt_gemm_bf16_split", nv.c_int, [nv._P, nv._P, nv._P, nv.c_int, nv.c_int, nv.c_int, nv.c_int, nv.c_int, nv._P,
+                                             nv.c_int, nv._P])
+nv.declare("mmt_sum_runs", nv.c_int, [nv._P, nv.c_int, nv._P, nv.c_int, nv.c_int, nv._P, nv._P])
 nv.declare("mmt_distill_scale", nv.c_int, [nv._P, nv.c_int, nv.c_long, nv._P, nv._P])
 
 
@@ -395,6 +399,22 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     return _DistillFn.apply(_rows(rows), ids, teacher, labels, float(temperature), float(label_weight), vocab_lo, group)
 
 
+def _gemm_over_vocab(grad, weight, out, count) -> None:
+    """``out[r] = grad[r] @ weight`` for as many rows as ``count[0]``.  A few rows have few tiles, each with the whole
+    vocabulary as its K: then the vocabulary is cut into runs, whose fp32 results are added up."""
+    from . import functional as F
+    rows, V = grad.shape
+    H = weight.shape[1]
+    runs = nv.lib().mmt_gemm_split(rows, H, V)
+    if runs < 2:
+        F._gemm_counted(grad, weight, out, count, b_mn=True)
+        return
+    parts = torch.empty(runs, rows, H, device=grad.device, dtype=torch.float32)
+    nv.call("mmt_gemm_bf16_split", grad.data_ptr(), weight.data_ptr(), parts.data_ptr(), rows, H, V, grad.stride(0),
+            weight.stride(0), count.data_ptr(), runs, nv.stream())
+    nv.call("mmt_sum_runs", parts.data_ptr(), runs, count.data_ptr(), rows, H, out.data_ptr(), nv.stream())
+
+
 def _head_pass(hidden, weight, teacher, temperature, share, vocab_lo, group, chunk_rows, need_h, dw, add):
     """Loss, and the gradient of ``hidden`` (if ``need_h``) and of ``weight`` (into ``dw``, on top of it if ``add``).
 
@@ -434,7 +454,7 @@ def _head_pass(hidden, weight, teacher, temperature, share, vocab_lo, group, chu
         else:
             d.both(logits, grad, src[c0:], n)
         if need_h:
-            F._gemm_counted(grad, weight, dx[c0:c1], n, b_mn=True)
+            _gemm_over_vocab(grad, weight, dx[c0:c1], n)
         if dw is not None:
             F._gemm_counted(grad, h, dw, n, of_k=True, a_mn=True, b_mn=True, accumulate=add or c0 > 0)
     return d.loss(), F.gather_rows_raw(dx, pos) if need_h else None
