@@ -199,6 +199,24 @@ class TextDecoder(nn.Module):
         return F.lm_head_cross_entropy(hg, w, shifted_labels, self.vocab_lo, self.tp.group, chunk_rows,
                                        label_smoothing=label_smoothing)
 
+    def distillation_loss(self, x_shard: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
+                          temperature: float = 1.0, shifted_labels: torch.Tensor | None = None, label_weight: float = 0.0,
+                          chunk_rows: int = 4096) -> torch.Tensor:
+        """:meth:`loss` against a teacher's top logits ([T, k] of all T tokens, :meth:`top_logits` of the teacher): row t's
+        are those behind token t, which predict the next one, as the shifted labels do."""
+        h = F.rmsnorm(x_shard, self.norm_w, self.cfg.rms_norm_eps)
+        hg = comm.all_gather(h, self.tp.group)
+        w = self.embed_tokens if self.lm_head is None else self.lm_head
+        return F.lm_head_distillation(hg, w, teacher_ids, teacher_logits, temperature=temperature, labels=shifted_labels,
+                                      label_weight=label_weight, vocab_lo=self.vocab_lo, group=self.tp.group,
+                                      chunk_rows=chunk_rows)
+
+    @torch.no_grad()
+    def top_logits(self, x_shard: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """What a student is taught of this model: the k largest logits behind every token and their ids, ([T, k], [T, k])
+        of the whole vocabulary on every rank."""
+        return F.top_logits(self.logits(x_shard), k, vocab_lo=self.vocab_lo, group=self.tp.group)
+
     def logits(self, x_shard: torch.Tensor) -> torch.Tensor:
         """Local vocab-shard logits [T, V/tp] (tests and evaluation)."""
         h = F.rmsnorm(x_shard, self.norm_w, self.cfg.rms_norm_eps)

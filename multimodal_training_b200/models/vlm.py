@@ -9,8 +9,9 @@ and as a single-process oracle of the disaggregated pipeline in the tests.
   images, writes the merged vision tokens over the image placeholders (the reference's ``masked_scatter`` at
   modeling_qwen2_5_vl.py:1858-1872), builds the 3-axis M-RoPE ids and runs the decoder.
 * ``loss`` is the shifted causal cross-entropy with ``-100`` ignored (mean over valid tokens).
-* ``generate`` is greedy decoding that recomputes the prefix each step (no KV cache): enough for evaluation
-  of short answers and for tests, not a serving path.
+* ``generate`` is decoding that recomputes the prefix each step (no KV cache): enough for evaluation of short answers and
+  for tests, not a serving path.  With a draft model, one pass of this model checks several drafted tokens.
+* ``top_logits`` and the ``teacher_*`` arguments of ``forward``: this model as a teacher, and as its student.
 """
 from __future__ import annotations
 
@@ -19,6 +20,7 @@ import torch.nn as nn
 
 from ..config.model_configs import VLConfig, get_model_config
 from ..data.rope_utils import get_rope_index_for_images
+from ..ops import functional as F
 from ..ops.attention import SeqInfo
 from ..parallel.sp import build_vision_plan
 from .text import TextDecoder, mrope_cos_sin
@@ -117,10 +119,14 @@ class Qwen2_5_VLForConditionalGeneration(nn.Module):
         self.config = self.model.config
 
     def forward(self, input_ids, pixel_values=None, image_grid_thw=None, attention_mask=None, labels=None,
-                **video_kw):
-        """Returns ``{"logits": [T, V]}`` and, with labels [B, S], ``"loss"`` (next-token CE, -100 ignored)."""
+                teacher_ids=None, teacher_logits=None, temperature: float = 1.0, label_weight: float = 0.0, **video_kw):
+        """Returns ``{"logits": [T, V]}`` and, with labels [B, S], ``"loss"`` (next-token CE, -100 ignored).
+
+        With ``teacher_ids`` and ``teacher_logits`` ([T, k] of the kept tokens, a teacher's :meth:`top_logits`), ``"loss"``
+        is that of :func:`..ops.functional.distillation_loss`: ``label_weight`` of it comes from the labels."""
         h, cu, keep = self.model.hidden_states(input_ids, pixel_values, image_grid_thw, attention_mask, **video_kw)
         out = {"logits": self.model.language_model.logits(h)}
+        shifted = None
         if labels is not None:
             if labels.dim() == 1:
                 labels = labels.unsqueeze(0)
@@ -129,13 +135,38 @@ class Qwen2_5_VLForConditionalGeneration(nn.Module):
             # the last kept token of every sample has nothing to predict
             lens = keep.sum(1)
             shifted[torch.arange(labels.shape[0]), (lens - 1).clamp(min=0)] = -100
-            out["loss"] = self.model.language_model.loss(h, shifted[keep].to(h.device))
+            shifted = shifted[keep].to(h.device)
+        if teacher_ids is not None:
+            out["loss"] = self.model.language_model.distillation_loss(
+                h, teacher_ids.to(h.device), teacher_logits.to(h.device), temperature=temperature, shifted_labels=shifted,
+                label_weight=label_weight)
+        elif shifted is not None:
+            out["loss"] = self.model.language_model.loss(h, shifted)
         return out
 
     @torch.no_grad()
+    def top_logits(self, k: int, input_ids, pixel_values=None, image_grid_thw=None, attention_mask=None, **video_kw):
+        """The k largest logits behind every kept token and their ids, ([T, k], [T, k]).  Rows that predict an image or video
+        token, and the last one of every sample, are no teacher: their ids are -1."""
+        h, cu, keep = self.model.hidden_states(input_ids, pixel_values, image_grid_thw, attention_mask, **video_kw)
+        values, ids = self.model.language_model.top_logits(h, k)
+        tokens = (input_ids if input_ids.dim() == 2 else input_ids.unsqueeze(0))[keep]
+        none = torch.zeros_like(tokens, dtype=torch.bool)
+        none[:-1] = (tokens[1:] == self.config.image_token_id) | (tokens[1:] == self.config.video_token_id)
+        none[[e - 1 for s, e in zip(cu, cu[1:]) if e > s]] = True
+        return values, ids.masked_fill(none.to(ids.device).unsqueeze(1), -1)
+
+    @torch.no_grad()
     def generate(self, input_ids, pixel_values=None, image_grid_thw=None, max_new_tokens: int = 16,
-                 eos_token_id: int | None = None) -> torch.Tensor:
-        """Greedy continuation of ONE sample; returns the full id sequence [S + new]."""
+                 eos_token_id: int | None = None, *, temperature: float = 0.0, generator: torch.Generator | None = None,
+                 draft_model: "Qwen2_5_VLForConditionalGeneration | None" = None, draft_tokens: int = 4) -> torch.Tensor:
+        """Continuation of ONE sample; returns the full id sequence [S + new].  Greedy, or drawn at ``temperature`` (random
+        numbers from ``generator``).  A ``draft_model`` with the same vocabulary proposes up to ``draft_tokens`` tokens,
+        which one pass of this model checks (:func:`..ops.functional.verify_drafts`): the answer has the distribution that
+        it has without a draft model, and is the same when greedy, up to the rounding of logits in passes of another length."""
+        if draft_model is not None or temperature > 0.0:
+            return self._generate_checked(input_ids, pixel_values, image_grid_thw, max_new_tokens, eos_token_id, temperature,
+                                          generator, draft_model, draft_tokens)
         ids = input_ids.flatten().clone()
         for _ in range(max_new_tokens):
             logits = self.model(ids.unsqueeze(0), pixel_values, image_grid_thw)
@@ -143,6 +174,42 @@ class Qwen2_5_VLForConditionalGeneration(nn.Module):
             ids = torch.cat([ids, torch.tensor([nxt], dtype=ids.dtype, device=ids.device)])
             if eos_token_id is not None and nxt == eos_token_id:
                 break
+        return ids
+
+    def _generate_checked(self, input_ids, pixel_values, image_grid_thw, max_new_tokens, eos_token_id, temperature, generator,
+                          draft_model, draft_tokens) -> torch.Tensor:
+        cfg = self.config
+        if draft_model is not None and draft_model.config.text.vocab_size != cfg.text.vocab_size:
+            raise ValueError(f"the draft model's vocabulary ({draft_model.config.text.vocab_size}) is not this model's "
+                             f"({cfg.text.vocab_size})")
+        if draft_model is not None and draft_tokens < 1:
+            raise ValueError("a draft model proposes at least one token")
+        ids = input_ids.flatten().clone()
+        images = () if pixel_values is None else (pixel_values, image_grid_thw)
+        stop = ids.numel() + max_new_tokens
+
+        def uniforms(n, like):
+            return torch.rand(1, n, generator=generator, device=like.device) if temperature > 0.0 else None
+
+        while ids.numel() < stop:
+            rows, seq = [], ids
+            for _ in range(min(draft_tokens, stop - ids.numel() - 1) if draft_model is not None else 0):
+                row = draft_model.model(seq.unsqueeze(0), *images)[-1:].to(self.model.language_model.embed_tokens.dtype)
+                # a placeholder has no rows of its own in the next pass
+                row[:, [cfg.image_token_id, cfg.video_token_id]] = -float("inf")
+                drawn = F.verify_drafts(row[None], torch.empty(1, 0, dtype=torch.int64, device=row.device), None,
+                                        uniforms(1, row), temperature=temperature)
+                rows.append(row)
+                seq = torch.cat([seq, drawn.tokens[0].to(seq)])
+            n = len(rows)
+            target = self.model(seq.unsqueeze(0), *images)[-(n + 1):].unsqueeze(0)
+            drafts = seq[ids.numel():].unsqueeze(0).to(target.device)
+            draft_logits = torch.cat(rows).unsqueeze(0) if n and temperature > 0.0 else None
+            r = F.verify_drafts(target, drafts, draft_logits, uniforms(n + 1, target), temperature=temperature)
+            new = r.tokens[0, :int(r.accepted) + 1].to(ids)
+            if eos_token_id is not None and bool((new == eos_token_id).any()):
+                return torch.cat([ids, new[:int((new == eos_token_id).nonzero()[0]) + 1]])
+            ids = torch.cat([ids, new])
         return ids
 
     def load_merged_state_dict(self, state: dict) -> None:
