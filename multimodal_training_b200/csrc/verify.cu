@@ -195,27 +195,30 @@ struct DrawShared {
 // 2^(x scale / 16 - whole / 16) in fp64, for a whole number `whole` near the largest x scale of the row: x scale - whole = n + f
 // with a whole n and |f| <= 1/2; 2^(n / 16) from a table of 16 (one word of each bank: no conflicts) and the exponent, 2^(f / 16)
 // by its series, whose rest is 2e-13 of it (Tang, Table-driven implementation of the exponential function, 1989).  Nine fp64
-// instructions and no branches: the drawn rows are bound by them.
+// instructions and no branches: what bounds the drawn rows is how many instructions a power takes.  The row is a distribution:
+// its largest logit is finite and none is not a number.  Logits 900 powers of two below the largest, -inf too, count as that
+// far below, which is nothing (kNothing).
 struct Powers16 {
   static constexpr double kMagic = 6755399441055744.0;    // 1.5 * 2^52: a number near it is rounded to a whole one
   double scale, shift;                            // shift = kMagic - whole
-  MMT_DEVICE Powers16(double scale_, double largest) : scale(scale_), shift(kMagic - rint(largest * scale_)) {}
+  float least;
+  MMT_DEVICE Powers16(double scale_, double largest)
+      : scale(scale_), shift(kMagic - rint(largest * scale_)), least((float)(largest - 16.0 * 900.0 / scale_)) {}
   MMT_DEVICE double of(float x, const double* table) const {
     constexpr double L = 0.69314718055994530942 / 16.0, L2 = L * L;
-    const double shifted = fma((double)x, scale, shift), f = fma((double)x, scale, shift - shifted);
+    const double d = (double)fmaxf(x, least), shifted = fma(d, scale, shift), f = fma(d, scale, shift - shifted);
     const int n = __double2loint(shifted);
     double p = fma(L2 * L2 * L / 120.0, f, L2 * L2 / 24.0);
     p = fma(p, f, L2 * L / 6.0);
     p = fma(p, f, L2 / 2.0);
     p = fma(p, f, L);
     const double t = table[n & 15], e = fma(t, p * f, t);
-    const double power = __hiloint2double(__double2hiint(e) + ((n >> 4) << 20), __double2loint(e));
-    const double some = shifted > kMagic - 16000.0 ? power : 0.0;         // none below 2^-1000
-    return x == x ? some : (double)x;
+    return __hiloint2double(__double2hiint(e) + ((n >> 4) << 20), __double2loint(e));
   }
 };
 
 // Weights of the columns of a row that a token is drawn from.
+constexpr double kNothing = 0x1p-800;             // a weight or a sum that is none
 enum Draw { kPlain, kWithout, kRest };            // p; p without one id; max(p - q, 0)
 template <typename T>
 struct Weigher {
@@ -227,8 +230,8 @@ struct Weigher {
   long x;
   Draw kind;
   MMT_DEVICE double rest(T xp, T xq) const {
-    const double d = of_p.of(to_float(xp), table) * by_p - of_q.of(to_float(xq), table) * by_q, r = d > 0.0 ? d : 0.0;
-    return d == d ? r : d;
+    const double d = of_p.of(to_float(xp), table) * by_p - of_q.of(to_float(xq), table) * by_q;
+    return d > 0.0 ? d : 0.0;
   }
   MMT_DEVICE double of(T xp, int c) const {
     if (kind == kRest) return rest(xp, q[c]);
@@ -423,13 +426,16 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(Verify v) 
   }
 
   // ---- the next token
-  const double m_p = row_sum(a).x;
+  // a row of the target that is no distribution draws nothing, one of the draft model leaves the target's
+  const double2 of_row = row_sum(a), of_draft = a < len && v.draft ? row_sum(n + 1 + a) : make_double2(0.0, 1.0);
+  const double m_p = of_row.x, m_q = of_draft.x;
+  auto distribution = [](double2 r) { return fabs(r.x) < INFINITY && r.y > 0.0 && r.y < INFINITY; };
+  const bool sound = distribution(of_row);
   Weigher<T> w = {target_row<T>(v, b, a), nullptr, s.table, Powers16(scale, m_p), Powers16(scale, m_p), 1.0, 1.0, -1, kPlain};
-  if (a < len) {
+  if (a < len && sound && distribution(of_draft)) {
     w.kind = kWithout;
     w.x = v.draft_ids[(long)b * n + a];
     if (v.draft) {
-      const double m_q = row_sum(n + 1 + a).x;
       const double2 sums = exact_sums(a, true, m_p, m_q);
       w.kind = kRest;
       w.q = draft_row<T>(v, b, a).p;
@@ -444,11 +450,11 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(Verify v) 
   auto warp_run = [&](int k) { return make_int2(min(run.x + k * share, run.y), min(run.x + (k + 1) * share, run.y)); };
   double rest = 0.0;                               // weight up to the token, from this CTA's first vector on
   int owner = -1;
-  for (;;) {
+  while (sound) {
     const int2 mine = warp_run(warp);
     const double part = block_sum(w.sum_run(mine.x + lane, mine.y, 32));
     const double total = cluster_total(make_double2(part, 0.0)).x;
-    if (!(total > 0.0)) {
+    if (!(total > kNothing)) {
       if (w.kind == kPlain) break;
       w.kind = kPlain;                              // no mass but the draft's: from the target itself
       continue;
@@ -458,7 +464,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(Verify v) 
     double up_to = 0.0;
     for (int k = 0; k < C && !(owner >= 0 && up_to > goal); ++k) {
       const double x = reinterpret_cast<const double2*>(&s.cta_part[turn ^ 1][k])->x;
-      if (!(x > 0.0)) continue;
+      if (!(x > kNothing)) continue;
       owner = k;
       rest = goal - up_to;
       up_to += x;
@@ -473,7 +479,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(Verify v) 
     double up_to = 0.0, from = 0.0;
     for (int q = 0; q < kDrawWarps && !(k >= 0 && up_to > rest); ++q) {
       const double x = s.warp_total[q];
-      if (!(x > 0.0)) continue;
+      if (!(x > kNothing)) continue;
       k = q;
       from = up_to;
       up_to += x;
@@ -495,7 +501,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(Verify v) 
       const double y = __shfl_up_sync(0xffffffffu, up_to, o);
       if (lane >= o) up_to += y;
     }
-    const uint32_t past = __ballot_sync(0xffffffffu, up_to > rest && x > 0.0);
+    const uint32_t past = __ballot_sync(0xffffffffu, up_to > rest && x > kNothing);
     if (past) {
       if (lane != __ffs(past) - 1) return;
       double sum = up_to - x;
@@ -503,7 +509,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(Verify v) 
       for (int j = 0; j < Row<T>::kVec && !(chosen >= 0 && sum > rest); ++j) {
         const int col = w.p.column(i0 + lane) + j;
         const double y = col >= 0 && col < v.V ? w.of(w.p.p[col], col) : 0.0;
-        if (!(y > 0.0)) continue;
+        if (!(y > kNothing)) continue;
         chosen = col;
         sum += y;
       }
@@ -516,7 +522,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(Verify v) 
   if (lane == 0) {
     int col = min(w.p.column(fine.y), v.V) - 1;
     const int least = max(w.p.column(fine.x), 0);
-    while (col > least && !(w.of(w.p.p[col], col) > 0.0)) --col;
+    while (col > least && !(w.of(w.p.p[col], col) > kNothing)) --col;
     *token = col;
   }
 }
