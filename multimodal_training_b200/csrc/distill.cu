@@ -8,9 +8,10 @@
 // its logits are not read.  The vocabulary may be one shard of several: the statistics of a row are then reduced over the
 // ranks between the kernels.
 //
-// Powers of two: with c = log2(e) / tau rounded to fp32, q_v = 2^(x_v c - top) / S, top = fl(max x * c), S = sum 2^(x c - top).
-// Statistics and gradient use the same rounded c and top, so their rounding changes the temperature by 2^-24 and
-// nothing else.  S is summed in fp32 (relative error of a few 2^-24); everything that is K long is fp64.
+// Powers of two: with c = log2(e) / tau rounded to fp32 and m the row's largest logit, q_v = 2^((x_v - m) c) / S,
+// S = sum 2^((x - m) c).  Statistics and gradient use the same rounded c, which changes the temperature by 2^-24 and nothing
+// else; the difference is taken first, so any finite logits do, the lowest of their type among them.  S is summed in fp32
+// (relative error of a few 2^-24); everything that is K long is fp64.
 #include "vocab_rows.cuh"
 
 namespace {
@@ -40,8 +41,7 @@ struct DistillCall {
   float temperature, share;
 };
 
-// Per row, in statistics of [kStats][rows]: top and top1 = fl(max x * c1), S and S1, the label's logit if it is in this
-// shard, sum of p x over the slots of this shard.  Or parts of the row's loss, one from each CTA that has worked on it.
+// Per row, in statistics of [kStats][rows]: m c and m c1, S and S1, the label's logit if it is in this shard, sum of p x over the slots of this shard.  Or parts of the row's loss, one from each CTA that has worked on it.
 constexpr int kMaxCluster = 8;
 enum { kTop, kTop1, kSum, kSum1, kLabel, kDot, kStats = kMaxCluster };
 
@@ -184,6 +184,9 @@ MMT_DEVICE Weights call_weights(const DistillRows& rows, const DistillCall& call
   return {(1.0 - (double)call.share) / max(t, 1), (double)call.share / max(l, 1)};
 }
 
+// What a sum of powers below `m` is worth below `top`; nothing for a set of nothing but -inf.
+MMT_DEVICE float rescale(float m, float c, float top) { return m == -INFINITY ? 0.f : pow2((m - top) * c); }
+
 // ----------------------------------------------------------------------------
 // Statistics of this shard's logits, one CTA per row.  With compacted rows (`src`: the row that each place holds, `cnt`:
 // places that are taken) logits go by place, everything else by row.
@@ -214,23 +217,22 @@ __global__ void __launch_bounds__(kDistillThreads) distill_stats_kernel(const T*
 #pragma unroll
     for (int j = 1; j < Row<T>::kVec; ++j) lm = fmaxf(lm, v[j]);
     if (lm > m) {
-      s *= exp2f(__fmul_rn(m, call.c) - __fmul_rn(lm, call.c));
-      if (kDual) s1 *= exp2f(__fmul_rn(m, call.c1) - __fmul_rn(lm, call.c1));
+      s *= rescale(m, call.c, lm);
+      if (kDual) s1 *= rescale(m, call.c1, lm);
       m = lm;
     }
     // a thread that has seen nothing but -inf adds zeros (2^-inf), not 2^(-inf + inf)
-    const float t = m == -INFINITY ? 0.f : __fmul_rn(m, call.c), t1 = m == -INFINITY ? 0.f : __fmul_rn(m, call.c1);
+    const float less = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int j = 0; j < Row<T>::kVec; ++j) {
-      s += exp2f(__fmaf_rn(v[j], call.c, -t));
-      if (kDual) s1 += exp2f(__fmaf_rn(v[j], call.c1, -t1));
+      s += pow2((v[j] - less) * call.c);
+      if (kDual) s1 += pow2((v[j] - less) * call.c1);
     }
   }
   const float gm = block_top<kDistillThreads>(m, red);
-  const float t = __fmul_rn(gm, call.c), t1 = __fmul_rn(gm, call.c1);
-  if (gm != -INFINITY) {                                       // 0 * 2^-inf for a thread without a logit
-    s *= exp2f(__fmul_rn(m, call.c) - t);
-    if (kDual) s1 *= exp2f(__fmul_rn(m, call.c1) - t1);
+  if (gm != -INFINITY) {
+    s *= rescale(m, call.c, gm);
+    if (kDual) s1 *= rescale(m, call.c1, gm);
   }
   s = block_total<kDistillThreads>(s, red);
   if (kDual) s1 = block_total<kDistillThreads>(s1, red);
@@ -246,8 +248,8 @@ __global__ void __launch_bounds__(kDistillThreads) distill_stats_kernel(const T*
   dot = block_total<kDistillThreads>(dot, dred);
   label = block_total<kDistillThreads>(label, dred);
   if (threadIdx.x == 0) {
-    stats[kTop * n_rows + at] = t;
-    stats[kTop1 * n_rows + at] = t1;
+    stats[kTop * n_rows + at] = (double)gm * (double)call.c;
+    stats[kTop1 * n_rows + at] = (double)gm * (double)call.c1;
     stats[kSum * n_rows + at] = s;
     stats[kSum1 * n_rows + at] = kDual ? s1 : s;
     stats[kDot * n_rows + at] = dot;
@@ -286,7 +288,7 @@ __global__ void __launch_bounds__(kDistillThreads) distill_grad_kernel(const T* 
   const float d = dloss ? *dloss : 1.f;
   const float wt = mark & kTaught ? (float)(w.taught * (double)call.temperature) * d : 0.f;
   const float wl = mark & kLabelled ? (float)w.labelled * d : 0.f;
-  const float t = (float)stats[kTop * n_rows + at], t1 = (float)stats[kTop1 * n_rows + at];
+  const float m = (float)(stats[kTop * n_rows + at] / (double)call.c);
   const float a = (kDual ? wt : wt + wl) / (float)stats[kSum * n_rows + at];
   const float a1 = kDual ? wl / (float)stats[kSum1 * n_rows + at] : 0.f;
   for (int j = threadIdx.x; j <= rows.K; j += kDistillThreads) {
@@ -299,8 +301,8 @@ __global__ void __launch_bounds__(kDistillThreads) distill_grad_kernel(const T* 
     RowVec<T>::unpack(row.load(i), v);
 #pragma unroll
     for (int j = 0; j < Row<T>::kVec; ++j) {
-      float g = a * exp2f(__fmaf_rn(v[j], call.c, -t));
-      if (kDual) g += a1 * exp2f(__fmaf_rn(v[j], call.c1, -t1));
+      float g = a * pow2((v[j] - m) * call.c);
+      if (kDual) g += a1 * pow2((v[j] - m) * call.c1);
       v[j] = g;
     }
     row.store(o, o_lead, i, v);
@@ -309,8 +311,8 @@ __global__ void __launch_bounds__(kDistillThreads) distill_grad_kernel(const T* 
   for (int j = threadIdx.x; j <= rows.K; j += kDistillThreads) {
     const long id = rows.slot_id[at * (rows.K + 1) + j];
     if (id < 0 || id < vocab_lo || id >= vocab_lo + V) continue;
-    float g = a * exp2f(__fmaf_rn(slot_x[j], call.c, -t));
-    if (kDual) g += a1 * exp2f(__fmaf_rn(slot_x[j], call.c1, -t1));
+    float g = a * pow2((slot_x[j] - m) * call.c);
+    if (kDual) g += a1 * pow2((slot_x[j] - m) * call.c1);
     g -= wt * rows.slot_p[at * (rows.K + 1) + j];
     if ((mark & kLabelled) && j == mark >> kSlotShift) g -= wl;
     from_float(g, o + (id - vocab_lo));
@@ -324,7 +326,7 @@ __global__ void __launch_bounds__(kDistillThreads) distill_grad_kernel(const T* 
 // once and its gradient written once.
 //
 // Second softmax (kMode): none, or that of temperature one for the labels.  If the temperature is a power of two, its powers
-// are the first one's squared log2(tau) times (c1 = tau c and top1 = tau top exactly).
+// are the first one's squared log2(tau) times (c1 = tau c exactly).
 //
 // The parts travel as asynchronous stores that count themselves into an mbarrier of the CTA they go to (two of them, in
 // turn: a CTA may be a row ahead of another, never two).  A barrier of the cluster would also wait until the gradients that
@@ -335,21 +337,20 @@ __global__ void __launch_bounds__(kDistillThreads) distill_grad_kernel(const T* 
 // ----------------------------------------------------------------------------
 constexpr int kSingle = 0, kSquares = 1, kTwice = 2;
 
-// 2^(a - b) for two tops, 0 for a set without any mass.
-MMT_DEVICE float rescale(float m, float c, float top) { return m == -INFINITY ? 0.f : pow2(__fmul_rn(m, c) - top); }
 
-// The two powers of two logits, with c = (c, c) and so on.
+// The two powers of two logits below `m`, with c = (c, c) and so on.
 struct Powers {
-  f32x2 c, c1, less, less1;               // less = (-top, -top)
+  f32x2 c, c1, less;
   int squares;
-  MMT_DEVICE Powers(const DistillCall& call, float t, float t1, int squares_)
-      : c(both(call.c, call.c)), c1(both(call.c1, call.c1)), less(both(-t, -t)), less1(both(-t1, -t1)), squares(squares_) {}
+  MMT_DEVICE Powers(const DistillCall& call, float m, int squares_)
+      : c(both(call.c, call.c)), c1(both(call.c1, call.c1)), less(both(-m, -m)), squares(squares_) {}
   template <int kMode>
   MMT_DEVICE void take(f32x2 x, f32x2& e, f32x2& e1) const {
-    float2 v = apart(fma2(x, c, less));
+    x = add2(x, less);
+    float2 v = apart(mul2(x, c));
     e = both(pow2(v.x), pow2(v.y));
     if constexpr (kMode == kTwice) {
-      v = apart(fma2(x, c1, less1));
+      v = apart(mul2(x, c1));
       e1 = both(pow2(v.x), pow2(v.y));
     }
     if constexpr (kMode == kSquares) {
@@ -454,10 +455,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       for (int i = tid; i < n; i += kThreads) m = thread_max(held[i], m, T());
       m = warp_top(m);
       // a warp that has nothing but -inf adds zeros (2^-inf), not 2^(-inf + inf)
-      const float t = m == -INFINITY ? 0.f : __fmul_rn(m, call.c), t1 = m == -INFINITY ? 0.f : __fmul_rn(m, call.c1);
       f32x2 s2 = both(0.f, 0.f), s12 = s2;
       {
-        const Powers pw(call, t, t1, squares);
+        const Powers pw(call, m == -INFINITY ? 0.f : m, squares);
 #pragma unroll 2
         for (int i = tid; i < n; i += kThreads) {
           float v[kVec];
@@ -482,8 +482,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       if (mark != 0) {
         a = warp_part[lane % kWarps];
         const float top = warp_top(a.x);
-        a.y *= rescale(a.x, call.c, __fmul_rn(top, call.c));
-        if constexpr (kDual) a.z *= rescale(a.x, call.c1, __fmul_rn(top, call.c1));
+        a.y *= rescale(a.x, call.c, top);
+        if constexpr (kDual) a.z *= rescale(a.x, call.c1, top);
         a.x = top;
 #pragma unroll
         for (int q = kWarps / 2; q > 0; q >>= 1) {
@@ -507,8 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       // lane q of every warp takes CTA q's part
       const float4 part = cta_part[turn][lane % C];
       const float top = warp_top(part.x);
-      const float t = __fmul_rn(top, call.c), t1 = __fmul_rn(top, call.c1);
-      float S = part.y * rescale(part.x, call.c, t), S1 = kDual ? part.z * rescale(part.x, call.c1, t1) : 0.f;
+      float S = part.y * rescale(part.x, call.c, top), S1 = kDual ? part.z * rescale(part.x, call.c1, top) : 0.f;
       for (int q = C / 2; q > 0; q >>= 1) {
         S += __shfl_xor_sync(0xffffffffu, S, q);
         if constexpr (kDual) S1 += __shfl_xor_sync(0xffffffffu, S1, q);
@@ -516,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       const int label_at = mark & kLabelled ? mark >> kSlotShift : -1;
       const float wt = mark & kTaught ? w_taught : 0.f, wl = mark & kLabelled ? w_labelled : 0.f;
       const float a = (kDual ? wt : wt + wl) / S, a1 = kDual ? wl / S1 : 0.f;
-      const Powers pw(call, t, t1, squares);
+      const Powers pw(call, top, squares);
       const f32x2 a2 = both(a, a), a12 = both(a1, a1);
       auto grad = [&](float x, float y) {
         f32x2 e, e1;
@@ -569,11 +568,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       }
       double part_loss = 0.0;
       if (warp == kWarps - 1) {
-        const double lse = (double)t + log2((double)S), lse1 = kDual ? (double)t1 + log2((double)S1) : lse;
+        const double lse = log2((double)S), lse1 = kDual ? log2((double)S1) : lse;         // above m c
         for (int j = lane; j < K1; j += 32)
           if (held_slot(j, id, p, x)) {
-            if (!(p == 0.f)) part_loss += loss_taught * (double)p * (lse - (double)x * (double)call.c);
-            if (j == label_at) part_loss += loss_labelled * (lse1 - (double)x * (double)call.c1);
+            if (!(p == 0.f)) part_loss += loss_taught * (double)p * (lse - ((double)x - (double)top) * (double)call.c);
+            if (j == label_at) part_loss += loss_labelled * (lse1 - ((double)x - (double)top) * (double)call.c1);
           }
       }
       __syncthreads();                             // `held` may be written again; a slot's gradient was another thread's

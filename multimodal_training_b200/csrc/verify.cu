@@ -32,7 +32,7 @@ struct Verify {
   long* accepted;                     // [batch]
   long* tokens;                       // [batch, drafts + 1]
   float* accept_prob;                 // [batch, drafts]
-  unsigned long long* parts;          // [batch, rows, splits]: (largest logit, sum of 2^(x c - fl(largest c))) of each part of
+  unsigned long long* parts;          // [batch, rows, splits]: (largest logit, sum of 2^((x - largest) c)) of each part of
                                       // a row; without sampling the key of its largest logit
   double inv_temperature;
   int batch, drafts, V, is_f32, uniforms_f64, sampled;
@@ -57,7 +57,7 @@ template <typename T>
 MMT_DEVICE Row<T> draft_row(const Verify& v, int b, int i) {
   return Row<T>(reinterpret_cast<const T*>(v.draft) + b * v.draft_seq + i * v.draft_row, v.V);
 }
-// fp32 exponents are x c - fl(m c), as in the sums of csrc/distill.cu.
+// fp32 exponents are (x - m) c, as in the sums of csrc/distill.cu.
 MMT_DEVICE float scale_of(const Verify& v) { return (float)(kLog2e * v.inv_temperature); }
 
 // ----------------------------------------------------------------------------
@@ -128,12 +128,10 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(Verify v) {
   } else {
     const float c = scale_of(v);
     const f32x2 c2 = both(c, c);
-    float m = edge >= 0 ? to_float(row.p[edge]) : -INFINITY;
-    const float x0 = m;
-    m = warp_top(m);
-    float t = m == -INFINITY ? 0.f : __fmul_rn(m, c);
+    const float x0 = edge >= 0 ? to_float(row.p[edge]) : -INFINITY;
+    float m = warp_top(x0);
     // what is not a number makes the sum so, and a warp that has nothing but -inf adds zeros (2^-inf), not 2^(-inf + inf)
-    f32x2 s = both(edge >= 0 ? pow2(__fmaf_rn(x0, c, -t)) : 0.f, 0.f);
+    f32x2 s = both(edge >= 0 ? pow2((x0 - (m == -INFINITY ? 0.f : m)) * c) : 0.f, 0.f);
     for (int i0 = lo + warp * 32; i0 < hi; i0 += kRowAhead * kRowThreads) {
       uint4 u[kRowAhead];
       const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
@@ -148,30 +146,32 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(Verify v) {
       for (int k = 0; k < kRowAhead; ++k) top = thread_max(u[k], top, T());
       top = warp_top(top);
       if (top > m) {
-        const float less = __fmul_rn(top, c), by = m == -INFINITY ? 0.f : pow2(t - less);
+        const float by = m == -INFINITY ? 0.f : pow2((m - top) * c);
         s = mul2(s, both(by, by));
-        t = less;
         m = top;
       }
-      const f32x2 less2 = both(-t, -t);
+      const float less = m == -INFINITY ? 0.f : m;
+      const f32x2 less2 = both(-less, -less);
+      f32x2 few = both(0.f, 0.f);                  // of these vectors: 16 terms, which keeps the chain of roundings short
 #pragma unroll
       for (int k = 0; k < kRowAhead; ++k) {
         float x[kVec];
         RowVec<T>::unpack(u[k], x);
 #pragma unroll
         for (int j = 0; j < kVec; j += 2) {
-          const float2 e = apart(fma2(both(x[j], x[j + 1]), c2, less2));
-          s = add2(s, both(pow2(e.x), pow2(e.y)));
+          const float2 e = apart(mul2(add2(both(x[j], x[j + 1]), less2), c2));
+          few = add2(few, both(pow2(e.x), pow2(e.y)));
         }
       }
+      s = add2(s, few);
     }
     const float sum = warp_sum(apart(s).x + apart(s).y);
     if (lane == 0) warp_part[warp] = make_float2(m, sum);
     __syncthreads();
     if (warp == 0) {
       const float2 a = warp_part[lane % kWarps];
-      const float top = warp_top(a.x), less = __fmul_rn(top, c);
-      float part = a.x == -INFINITY ? a.y : a.y * pow2(__fmul_rn(a.x, c) - less);
+      const float top = warp_top(a.x);
+      float part = a.x == -INFINITY ? a.y : a.y * pow2((a.x - top) * c);
 #pragma unroll
       for (int o = kWarps / 2; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
       if (lane == 0) *reinterpret_cast<float2*>(out) = make_float2(top, part);
@@ -200,10 +200,16 @@ struct DrawShared {
 // far below, which is nothing (kNothing).
 struct Powers16 {
   static constexpr double kMagic = 6755399441055744.0;    // 1.5 * 2^52: a number near it is rounded to a whole one
-  double scale, shift;                            // shift = kMagic - whole
+  double scale, shift, largest;                   // shift = kMagic - whole
   float least;
-  MMT_DEVICE Powers16(double scale_, double largest)
-      : scale(scale_), shift(kMagic - rint(largest * scale_)), least((float)(largest - 16.0 * 900.0 / scale_)) {}
+  MMT_DEVICE Powers16(double scale_, double largest_)
+      : scale(scale_), shift(kMagic - rint(largest_ * scale_)), largest(largest_),
+        least((float)(largest_ - 16.0 * 900.0 / scale_)) {}
+  // Whether the largest logit is too far from zero for a whole number beside kMagic; such a row takes the long way.
+  MMT_DEVICE bool far() const { return fabs(largest) * scale > 0x1p45; }
+  MMT_DEVICE double any(float x, const double* table) const {
+    return far() ? exp2(((double)x - largest) * (scale / 16.0)) : of(x, table);
+  }
   MMT_DEVICE double of(float x, const double* table) const {
     constexpr double L = 0.69314718055994530942 / 16.0, L2 = L * L;
     const double d = (double)fmaxf(x, least), shifted = fma(d, scale, shift), f = fma(d, scale, shift - shifted);
@@ -234,14 +240,16 @@ struct Weigher {
     return d > 0.0 ? d : 0.0;
   }
   MMT_DEVICE double of(T xp, int c) const {
-    if (kind == kRest) return rest(xp, q[c]);
-    return kind == kWithout && c == x ? 0.0 : of_p.of(to_float(xp), table);
+    const double e = of_p.any(to_float(xp), table);
+    if (kind != kRest) return kind == kWithout && c == x ? 0.0 : e;
+    const double d = e * by_p - of_q.any(to_float(q[c]), table) * by_q;
+    return d > 0.0 ? d : 0.0;
   }
   // Sum over vector i, whose logits are `u` if it is a whole one.
   MMT_DEVICE double sum(int i, const uint4& u) const {
     const int c = p.column(i);
     double s = 0.0;
-    if (p.whole(i)) {
+    if (p.whole(i) && !of_p.far() && !of_q.far()) {
       if (kind == kRest && Row<T>::lead_of(q) == p.lead) {
         const uint4 uq = *reinterpret_cast<const uint4*>(q + c);
 #pragma unroll
@@ -304,11 +312,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(Verify v) 
     const float2 none = make_float2(-INFINITY, 0.f);
     const float2 x = lane < v.splits ? part[lane] : none, y = lane + 32 < v.splits ? part[lane + 32] : none;
     const float m = warp_top(fmaxf(x.x, y.x));
-    // a part's sum is relative to fl(its largest c)
-    auto of = [&](float2 p) {
-      const double less = (double)__fmul_rn(p.x, c) - (double)m * (double)c;
-      return p.x == -INFINITY ? (double)p.y : (double)p.y * exp2(less);
-    };
+    auto of = [&](float2 p) { return p.x == -INFINITY ? (double)p.y : (double)p.y * exp2(((double)p.x - (double)m) * (double)c); };
     return make_double2((double)m, warp_total_of(of(x) + of(y)));
   };
   // largest logit's id of a row without sampling; by a warp
@@ -405,8 +409,8 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(Verify v) 
       if (s.verdict[j] == kHangs) {
         const float2 x = s.logits[j], m = s.largest[j];
         const double2 sums = exact_sums(c0 + j, v.draft != nullptr, m.x, m.y);
-        const double q = v.draft ? Powers16(scale, m.y).of(x.y, s.table) / sums.y : 1.0;
-        falls = !(uniform(v, b, c0 + j) * q < Powers16(scale, m.x).of(x.x, s.table) / sums.x);
+        const double q = v.draft ? Powers16(scale, m.y).any(x.y, s.table) / sums.y : 1.0;
+        falls = !(uniform(v, b, c0 + j) * q < Powers16(scale, m.x).any(x.x, s.table) / sums.x);
       }
       if (falls) a = c0 + j;
     }

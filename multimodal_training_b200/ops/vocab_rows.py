@@ -294,6 +294,11 @@ class _DistillFn(torch.autograd.Function):
         return (grad,) + (None,) * 7
 
 
+# Temperatures beyond these are mistakes (of units, or a zero that was to mean greedy), and keep log2(e) / temperature and the
+# squares of both far from the ends of fp32.
+_COLDEST, _HOTTEST = 2.0 ** -20, 2.0 ** 20
+
+
 def _check_distill(shape, device, teacher_ids, teacher_logits, temperature, labels, label_weight):
     """Teacher and labels as the kernels take them: [rows, K] twice, [rows] or None."""
     if teacher_ids.shape != teacher_logits.shape or teacher_ids.dim() < 1 or teacher_ids.shape[:-1] != shape:
@@ -306,8 +311,8 @@ def _check_distill(shape, device, teacher_ids, teacher_logits, temperature, labe
     _floating(teacher_logits, "teacher_logits")
     if teacher_logits.requires_grad:
         raise ValueError("teacher_logits are data of the loss: detach them")
-    if not (temperature > 0.0 and math.isfinite(temperature)):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not _COLDEST <= temperature <= _HOTTEST:
+        raise ValueError(f"temperature must be positive, from 2^-20 to 2^20, got {temperature}")
     if not 0.0 <= label_weight <= 1.0:
         raise ValueError(f"label_weight must be in [0, 1], got {label_weight}")
     if label_weight > 0.0 and labels is None:
@@ -650,8 +655,8 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
         raise ValueError(f"target_logits {tuple(target_logits.shape)} do not have a row more than draft_ids ({B}, {n})")
     _floating(target_logits, "target_logits")
     _integral(draft_ids, "draft_ids")
-    if not (temperature >= 0.0 and math.isfinite(temperature)):
-        raise ValueError(f"temperature must be finite and not negative, got {temperature}")
+    if not (temperature == 0.0 or _COLDEST <= temperature <= _HOTTEST):
+        raise ValueError(f"temperature must be 0 (greedy) or from 2^-20 to 2^20, got {temperature}")
     if temperature == 0.0:
         if draft_logits is not None or uniforms is not None:
             raise ValueError("temperature 0 takes neither draft_logits nor uniforms")

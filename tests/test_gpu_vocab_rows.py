@@ -184,6 +184,26 @@ def test_distillation_of_unusual_rows(dtype):
     assert float(loss) == 0.0 and grad.shape == (0, V)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("temperature,share", [(1.0, 0.5), (2.0, 0.5), (3.0, 0.5)])
+def test_distillation_of_rows_masked_with_the_lowest_value(dtype, temperature, share):
+    T, V, K = 8, 1003, 4
+    low = torch.finfo(dtype).min
+    x, ids, teacher, labels = _batch(T, V, K, dtype)
+    ids[:], labels[:] = torch.arange(K, device="cuda"), 2
+    teacher[:] = torch.arange(K, device="cuda").float()
+    x[0, 10:] = low                                 # part of a row
+    x[1] = low                                      # all of it: every id is as likely
+    x[2] = -low
+    x[3] = 1e30
+    x[4, :] = 2e4
+    x[4, ::2] += 100
+    # what is masked has no part in the divergence here, so fp64 has an answer for all of them; its quotients by the
+    # temperature do not overflow
+    want = oracle.distill(x, ids, teacher, temperature, labels, share)
+    _near(*_loss_and_grad(x, ids, teacher, temperature=temperature, labels=labels, label_weight=share), *want, temperature, dtype)
+
+
 def test_ids_outside_the_vocabulary_are_left_out_and_reported():
     from multimodal_training_b200.ops import native as nv
     x, ids, teacher, labels = _batch(8, 300, 6, BF16)
@@ -292,7 +312,8 @@ def _same(got, want):
     prob = got.accept_prob.cpu()
     assert torch.equal(prob.isnan(), want[2].isnan())
     # the normalisers may be sums of fp32 terms: 2^-15 as above, for both models
-    assert ((prob.double() - want[2]).nan_to_num(0.0).abs() <= 2.0 ** -14 * want[2].nan_to_num(1.0)).all()
+    # (and the chance is returned in fp32, with what is below its smallest normal number, 2^-126, flushed to zero)
+    assert ((prob.double() - want[2]).nan_to_num(0.0).abs() <= 2.0 ** -14 * want[2].nan_to_num(1.0) + 2.0 ** -126).all()
 
 
 @pytest.mark.parametrize("B,n,V", [(1, 0, 1), (1, 4, 7), (3, 1, 1000), (40, 3, 1025), (2, 8, 50001), (2, 2, 152064), (70, 0, 4096)])
@@ -358,6 +379,26 @@ def test_verification_of_unusual_rows(dtype):
     none = torch.empty(4, 0, dtype=torch.int64, device="cuda")
     got = F.verify_drafts(greedy.to(dtype).cuda(), none, temperature=0.0)
     assert got.tokens[:, 0].tolist() == [0, 444, 699, 0]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("temperature", [0.0, 0.7, 1.0])
+def test_verification_of_rows_far_from_zero(dtype, temperature):
+    F = _ops()
+    V = 3001
+    low = torch.finfo(dtype).min
+    g = torch.Generator().manual_seed(4)
+    target = torch.randn(6, 2, V, generator=g)
+    draft = target[:, :1] + torch.randn(6, 1, V, generator=g)
+    target[0], draft[0, :, 5:] = low, low
+    target[1, :, ::2], draft[1] = low, low
+    target[2:4], draft[2:4] = 1e30 * target[2:4].round(), 1e30
+    target[4:], draft[4:] = 30000.0 + 64 * target[4:].round(), 30000.0
+    ids = torch.tensor([[3], [7], [9], [11], [12], [0]]).cuda()
+    u = torch.tensor([[0.9, 0.3]] * 6).cuda() if temperature else None
+    target, draft = target.to(dtype).cuda(), draft.to(dtype).cuda() if temperature else None
+    got = F.verify_drafts(target, ids, draft, u, temperature=temperature)
+    _same(got, oracle.verify(target, ids, draft, u, temperature))
 
 
 def test_rows_behind_a_shorter_draft_are_not_read():

@@ -135,7 +135,7 @@ def test_distillation_refusals():
     x, ids, teacher, labels = _batch(4, 11, 3)
     ok = dict(temperature=1.0, labels=labels, label_weight=0.5)
     F.distillation_loss(x, ids, teacher, **ok)
-    for bad in (dict(ok, temperature=0.0), dict(ok, temperature=-1.0), dict(ok, temperature=NAN), dict(ok, temperature=INF),
+    for bad in (dict(ok, temperature=0.0), dict(ok, temperature=1e-7), dict(ok, temperature=2e6), dict(ok, temperature=-1.0), dict(ok, temperature=NAN), dict(ok, temperature=INF),
                 dict(ok, label_weight=1.5), dict(ok, label_weight=-0.1), dict(ok, labels=None), dict(ok, labels=labels[:2])):
         with pytest.raises(ValueError):
             F.distillation_loss(x, ids, teacher, **bad)
@@ -291,7 +291,7 @@ def test_verification_refusals():
     for args in bad:
         with pytest.raises(ValueError):
             F.verify_drafts(*args)
-    for kw in (dict(temperature=-1.0), dict(temperature=NAN), dict(temperature=0.0), dict(draft_lens=torch.zeros(2, dtype=torch.int64))):
+    for kw in (dict(temperature=-1.0), dict(temperature=1e-7), dict(temperature=2e6), dict(temperature=NAN), dict(temperature=0.0), dict(draft_lens=torch.zeros(2, dtype=torch.int64))):
         with pytest.raises(ValueError):
             F.verify_drafts(target, ids, draft, u, **kw)
     for args in ((target.long(), ids, None, u), (target, ids.float(), draft, u), (target, ids, draft.double(), u),
