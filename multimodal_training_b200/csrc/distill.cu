@@ -41,9 +41,12 @@ struct DistillCall {
   float temperature, share;
 };
 
-// Per row, in statistics of [kStats][rows]: m c and m c1, S and S1, the label's logit if it is in this shard, sum of p x over the slots of this shard.  Or parts of the row's loss, one from each CTA that has worked on it.
+// Per row, in statistics of [kStats][rows], of this shard: m c and m c1, S and S1, (x - m) c1 of the label if it is here and
+// 1 then, sum of p (x - m) c and of p over the slots that are here.  Or parts of the row's loss, one from each CTA that has
+// worked on it, which start as zeros.
 constexpr int kMaxCluster = 8;
-enum { kTop, kTop1, kSum, kSum1, kLabel, kDot, kStats = kMaxCluster };
+enum { kTop, kTop1, kSum, kSum1, kLabel, kDot, kMass, kMine, kStats };
+static_assert(kStats == kMaxCluster, "the parts of a row's loss lie where its statistics do");
 
 // ----------------------------------------------------------------------------
 // Teacher's side: one warp per row.  An entry is absent if its id is negative or its logit -inf.
@@ -52,7 +55,7 @@ constexpr int kPrepareRows = 8;                    // warps of a block
 template <typename T>
 __global__ void __launch_bounds__(32 * kPrepareRows) distill_prepare_kernel(const long* ids, long ids_ld, const T* teacher,
                                                                             long teacher_ld, const long* labels, long rows,
-                                                                            long vocab, double inv_temperature,
+                                                                            long vocab, double inv_temperature, int taught,
                                                                             DistillRows out, long* need,
                                                                             double* stats, int* ticket,
                                                                             MmtErrorWord* ew) {
@@ -78,7 +81,7 @@ __global__ void __launch_bounds__(32 * kPrepareRows) distill_prepare_kernel(cons
         mmt_report(ew, MMT_ERR_BOUNDS, 700, (int)row);
         id = -1;
       }
-      const bool here = id >= 0 && !(t == -INFINITY);
+      const bool here = taught && id >= 0 && !(t == -INFINITY);
       s_id[warp][j] = here ? (int)id : -1;
       s_p[warp][j] = here ? (double)t * inv_temperature : -INFINITY;
       any |= here;
@@ -151,10 +154,10 @@ __global__ void __launch_bounds__(32 * kPrepareRows) distill_prepare_kernel(cons
       out.slot_p[row * (K + 1) + K] = 0.f;
       out.info[row] = any ? make_double2(dot * inv_total - log(total), sum_p) : make_double2(0.0, 0.0);
       out.mark[row] = mark;
-      if (need) need[row] = mark ? 0 : -1;
+      if (need) need[row] = mark ? row : -1;
     }
   }
-  if (row < rows && mark == 0 && lane < kStats) stats[lane * rows + row] = 0.0;      // such a row has no loss
+  if (row < rows && lane < kStats) stats[lane * rows + row] = 0.0;
   if (lane == 0) marks[warp] = mark;
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -203,10 +206,7 @@ __global__ void __launch_bounds__(kDistillThreads) distill_stats_kernel(const T*
   const long at = src ? src[blockIdx.x] : (long)blockIdx.x;
   if (at < 0) return;
   const int mark = rows.mark[at];
-  if (mark == 0) {
-    if (threadIdx.x <= kDot) stats[threadIdx.x * n_rows + at] = threadIdx.x == kSum || threadIdx.x == kSum1 ? 1.0 : 0.0;
-    return;
-  }
+  if (mark == 0) return;
   const Row<T> row(logits + blockIdx.x * ld, V);
   const int nv = row.vectors();
   float m = -INFINITY, s = 0.f, s1 = 0.f;
@@ -236,16 +236,24 @@ __global__ void __launch_bounds__(kDistillThreads) distill_stats_kernel(const T*
   }
   s = block_total<kDistillThreads>(s, red);
   if (kDual) s1 = block_total<kDistillThreads>(s1, red);
-  double dot = 0.0, label = 0.0;
+  const double zero_at = gm == -INFINITY ? 0.0 : (double)gm;
+  double dot = 0.0, mass = 0.0, label = 0.0;
+  int mine = 0;
   for (int j = threadIdx.x; j <= rows.K; j += kDistillThreads) {
     const long id = rows.slot_id[at * (rows.K + 1) + j];
     const float p = rows.slot_p[at * (rows.K + 1) + j];
     if (id < 0 || id < vocab_lo || id >= vocab_lo + V) continue;
-    const float x = to_float(row.p[id - vocab_lo]);
-    if (!(p == 0.f)) dot += (double)p * (double)x;
-    if ((mark & kLabelled) && j == mark >> kSlotShift) label = (double)x;
+    const double x = (double)to_float(row.p[id - vocab_lo]) - zero_at;
+    if (!(p == 0.f)) dot += (double)p * x * (double)call.c;
+    mass += (double)p;
+    if ((mark & kLabelled) && j == mark >> kSlotShift) {
+      label = x * (double)call.c1;
+      mine = 1;
+    }
   }
+  mine = __syncthreads_or(mine);
   dot = block_total<kDistillThreads>(dot, dred);
+  mass = block_total<kDistillThreads>(mass, dred);
   label = block_total<kDistillThreads>(label, dred);
   if (threadIdx.x == 0) {
     stats[kTop * n_rows + at] = (double)gm * (double)call.c;
@@ -254,11 +262,13 @@ __global__ void __launch_bounds__(kDistillThreads) distill_stats_kernel(const T*
     stats[kSum1 * n_rows + at] = kDual ? s1 : s;
     stats[kDot * n_rows + at] = dot;
     stats[kLabel * n_rows + at] = label;
+    stats[kMass * n_rows + at] = mass;
+    stats[kMine * n_rows + at] = (double)mine;
   }
 }
 
 // ----------------------------------------------------------------------------
-// Gradient from the whole vocabulary's statistics, one CTA per row, into `out` (which may be the logits).
+// Gradient from the whole vocabulary's statistics, one CTA per row, into `out`.
 // ----------------------------------------------------------------------------
 template <typename T, typename O, bool kDual>
 __global__ void __launch_bounds__(kDistillThreads) distill_grad_kernel(const T* logits, long ld, int V, long vocab_lo,
@@ -295,7 +305,7 @@ __global__ void __launch_bounds__(kDistillThreads) distill_grad_kernel(const T* 
     const long id = rows.slot_id[at * (rows.K + 1) + j];
     if (id >= 0 && id >= vocab_lo && id < vocab_lo + V) slot_x[j] = to_float(row.p[id - vocab_lo]);
   }
-  __syncthreads();                                            // the logits are written over below
+  __syncthreads();
   for (int i = threadIdx.x; i < nv; i += kDistillThreads) {
     float v[Row<T>::kVec];
     RowVec<T>::unpack(row.load(i), v);
@@ -332,11 +342,10 @@ __global__ void __launch_bounds__(kDistillThreads) distill_grad_kernel(const T* 
 // turn: a CTA may be a row ahead of another, never two).  A barrier of the cluster would also wait until the gradients that
 // the threads have stored are visible, which is several microseconds.
 //
-// Rows are handed out by tickets: a cluster knows its row and the next one, which is on its way into L2, and takes a ticket
-// for the one after that, which travels with the parts.
+// Rows are handed out by tickets: a cluster knows its row and the next one, whose copy starts as soon as the row's gradients
+// are formed, and takes a ticket for the one after that, which travels with the parts.
 // ----------------------------------------------------------------------------
 constexpr int kSingle = 0, kSquares = 1, kTwice = 2;
-
 
 // The two powers of two logits below `m`, with c = (c, c) and so on.
 struct Powers {
@@ -618,14 +627,11 @@ __global__ void __launch_bounds__(256) distill_row_loss_kernel(DistillRows rows,
   double loss = 0.0;
   if ((mark & kTaught) && w.taught > 0.0) {
     const double2 info = rows.info[r];
-    const double lse = stats[kTop * n_rows + r] + log2(stats[kSum * n_rows + r]);
-    const double kl = info.x - kLn2 * (stats[kDot * n_rows + r] * (double)call.c - info.y * lse);
+    const double kl = info.x - kLn2 * (stats[kDot * n_rows + r] - info.y * log2(stats[kSum * n_rows + r]));
     loss += w.taught * (double)call.temperature * (double)call.temperature * kl;
   }
-  if ((mark & kLabelled) && w.labelled > 0.0) {
-    const double lse = stats[kTop1 * n_rows + r] + log2(stats[kSum1 * n_rows + r]);
-    loss += w.labelled * kLn2 * (lse - stats[kLabel * n_rows + r] * (double)call.c1);
-  }
+  if ((mark & kLabelled) && w.labelled > 0.0)
+    loss += w.labelled * kLn2 * (log2(stats[kSum1 * n_rows + r]) - stats[kLabel * n_rows + r]);
   stats[r] = loss;
 }
 
@@ -753,7 +759,7 @@ constexpr int kHeldBytes = 40 * 1024, kMaxHeldBytes = 200 * 1024;
 
 template <typename T, typename O, int kThreads, int kMode>
 int launch_held(MmtDistill& d, int C, int per, int squares, void* stream) {
-  d.parts = C;
+  d.parts = max(d.parts, C);                // chunks of a batch differ in it
   auto kernel = distill_fused_kernel<T, O, kThreads, kMode>;
   static int allowed = 0;
   const int bytes = per * 16;
@@ -805,7 +811,7 @@ int mmt_distill_stats_count() { return kStats; }
 int mmt_distill_count_rows() { return kPrepareRows; }
 
 // Teacher's side of `rows` rows: ids [rows, K] and logits [rows, K] (bf16 or fp32), labels [rows] or null.
-// need [rows] or null: 0 for a row with a teacher or a label, -1 for one without.
+// need [rows] or null: the row itself if it has a teacher or a label, -1 for one without.
 int mmt_distill_prepare(const MmtDistill* d, const long* ids, long ids_ld, const void* teacher, long teacher_ld,
                         int teacher_f32, const long* labels, long vocab, long* need, void* stream) {
   if (wrong(*d) || vocab > 0x7fffffffL) return -2;
@@ -815,10 +821,10 @@ int mmt_distill_prepare(const MmtDistill* d, const long* ids, long ids_ld, const
   if (teacher_f32)
     return (int)launch_dependent(distill_prepare_kernel<float>, grid, 32 * kPrepareRows, 0, VR_STREAM(stream), ids, ids_ld,
                                  reinterpret_cast<const float*>(teacher), teacher_ld, labels, d->rows, vocab, inv,
-                                 rows_of(*d), need, d->stats, d->ticket, mmt_error_word());
+                                 (int)(d->share < 1.0), rows_of(*d), need, d->stats, d->ticket, mmt_error_word());
   return (int)launch_dependent(distill_prepare_kernel<bf16>, grid, 32 * kPrepareRows, 0, VR_STREAM(stream), ids, ids_ld,
-                               reinterpret_cast<const bf16*>(teacher), teacher_ld, labels, d->rows, vocab, inv, rows_of(*d),
-                               need, d->stats, d->ticket, mmt_error_word());
+                               reinterpret_cast<const bf16*>(teacher), teacher_ld, labels, d->rows, vocab, inv,
+                               (int)(d->share < 1.0), rows_of(*d), need, d->stats, d->ticket, mmt_error_word());
 }
 
 int mmt_distill_stats(MmtDistill* d, void* stream) {

@@ -225,6 +225,7 @@ struct Powers16 {
 
 // Weights of the columns of a row that a token is drawn from.
 constexpr double kNothing = 0x1p-800;             // a weight or a sum that is none
+constexpr double kNoRest = 0x1p-46;               // a sum of max(p - q, 0) that may be the rounding of p and q, 2^-53 a step
 enum Draw { kPlain, kWithout, kRest };            // p; p without one id; max(p - q, 0)
 template <typename T>
 struct Weigher {
@@ -458,7 +459,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(Verify v) 
     const int2 mine = warp_run(warp);
     const double part = block_sum(w.sum_run(mine.x + lane, mine.y, 32));
     const double total = cluster_total(make_double2(part, 0.0)).x;
-    if (!(total > kNothing)) {
+    if (!(total > (w.kind == kRest ? kNoRest : kNothing))) {
       if (w.kind == kPlain) break;
       w.kind = kPlain;                              // no mass but the draft's: from the target itself
       continue;

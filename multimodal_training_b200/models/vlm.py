@@ -161,10 +161,10 @@ class Qwen2_5_VLForConditionalGeneration(nn.Module):
                  eos_token_id: int | None = None, *, temperature: float = 0.0, generator: torch.Generator | None = None,
                  draft_model: "Qwen2_5_VLForConditionalGeneration | None" = None, draft_tokens: int = 4) -> torch.Tensor:
         """Continuation of ONE sample; returns the full id sequence [S + new].  Greedy, or drawn at ``temperature`` (random
-        numbers from ``generator``).  A ``draft_model`` with the same vocabulary proposes up to ``draft_tokens`` tokens,
+        numbers from ``generator``; image and video placeholders are not drawn).  A ``draft_model`` with the same vocabulary proposes up to ``draft_tokens`` tokens,
         which one pass of this model checks (:func:`..ops.functional.verify_drafts`): the answer has the distribution that
         it has without a draft model, and is the same when greedy, up to the rounding of logits in passes of another length."""
-        if draft_model is not None or temperature > 0.0:
+        if draft_model is not None or temperature != 0.0:
             return self._generate_checked(input_ids, pixel_values, image_grid_thw, max_new_tokens, eos_token_id, temperature,
                                           generator, draft_model, draft_tokens)
         ids = input_ids.flatten().clone()
@@ -184,6 +184,15 @@ class Qwen2_5_VLForConditionalGeneration(nn.Module):
                              f"({cfg.text.vocab_size})")
         if draft_model is not None and draft_tokens < 1:
             raise ValueError("a draft model proposes at least one token")
+        if temperature < 0.0:
+            raise ValueError(f"temperature must not be negative, got {temperature}")
+        placeholders = [cfg.image_token_id, cfg.video_token_id]
+
+        def checked(tokens):
+            if bool((tokens < 0).any()):
+                raise RuntimeError("logits that are no distribution (NaN, or all -inf): no token can be drawn")
+            return tokens.to(ids)
+
         ids = input_ids.flatten().clone()
         images = () if pixel_values is None else (pixel_values, image_grid_thw)
         stop = ids.numel() + max_new_tokens
@@ -196,17 +205,19 @@ class Qwen2_5_VLForConditionalGeneration(nn.Module):
             for _ in range(min(draft_tokens, stop - ids.numel() - 1) if draft_model is not None else 0):
                 row = draft_model.model(seq.unsqueeze(0), *images)[-1:].to(self.model.language_model.embed_tokens.dtype)
                 # a placeholder has no rows of its own in the next pass
-                row[:, [cfg.image_token_id, cfg.video_token_id]] = -float("inf")
+                row[:, placeholders] = -float("inf")
                 drawn = F.verify_drafts(row[None], torch.empty(1, 0, dtype=torch.int64, device=row.device), None,
                                         uniforms(1, row), temperature=temperature)
                 rows.append(row)
-                seq = torch.cat([seq, drawn.tokens[0].to(seq)])
+                seq = torch.cat([seq, checked(drawn.tokens[0])])
             n = len(rows)
             target = self.model(seq.unsqueeze(0), *images)[-(n + 1):].unsqueeze(0)
+            if temperature > 0.0:
+                target[..., placeholders] = -float("inf")
             drafts = seq[ids.numel():].unsqueeze(0).to(target.device)
             draft_logits = torch.cat(rows).unsqueeze(0) if n and temperature > 0.0 else None
             r = F.verify_drafts(target, drafts, draft_logits, uniforms(n + 1, target), temperature=temperature)
-            new = r.tokens[0, :int(r.accepted) + 1].to(ids)
+            new = checked(r.tokens[0, :int(r.accepted) + 1])
             if eos_token_id is not None and bool((new == eos_token_id).any()):
                 return torch.cat([ids, new[:int((new == eos_token_id).nonzero()[0]) + 1]])
             ids = torch.cat([ids, new])

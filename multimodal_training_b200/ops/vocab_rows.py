@@ -214,12 +214,17 @@ class _Distill:
         top = self.stats[:2, lo:hi].contiguous()
         mine = top.clone()
         F._all_reduce(top, torch.distributed.ReduceOp.MAX, group)
-        rest = self.stats[2:6, lo:hi].contiguous()
-        # a shard of nothing but -inf has a sum of zero, which stays
-        rest[:2] = torch.where(rest[:2] > 0, rest[:2] * torch.exp2(mine - top), rest[:2])
+        rest = self.stats[2:, lo:hi].contiguous()
+        sums, label, dot, mass, has_label = rest[:2], rest[2], rest[3], rest[4], rest[5]
+        # from below this shard's largest logit to below the whole vocabulary's; a shard of nothing but -inf has a sum of
+        # zero, which stays
+        down = mine - top
+        sums.copy_(torch.where(sums > 0, sums * torch.exp2(down), sums))
+        label.add_(torch.where(has_label > 0, down[1], 0.0))
+        dot.add_(torch.where(mass > 0, mass * down[0], 0.0))
         F._all_reduce(rest, torch.distributed.ReduceOp.SUM, group)
         self.stats[:2, lo:hi] = top
-        self.stats[2:6, lo:hi] = rest
+        self.stats[2:, lo:hi] = rest
 
     def _out(self, out, dloss=None) -> None:
         w = self.words
@@ -252,6 +257,12 @@ class _Distill:
         return out
 
 
+def _captured_with_forward(ctx) -> None:
+    """What an eager forward pass keeps is freed behind its backward pass, so that a replay would read anything."""
+    if torch.cuda.is_current_stream_capturing() and not ctx.captured:
+        raise RuntimeError("this backward pass is being captured into a graph, its forward pass was not: capture both")
+
+
 class _DistillFn(torch.autograd.Function):
     """The gradient is written in forward, while the row's statistics are at hand, and handed over by the first backward
     pass (times its ``dloss``, where that is not one).  Another backward pass, and one that is captured into a graph (a
@@ -268,7 +279,7 @@ class _DistillFn(torch.autograd.Function):
             if not torch.cuda.is_current_stream_capturing():
                 ctx.early = torch.empty(rows, V, device=logits.device, dtype=logits.dtype)
             ctx.save_for_backward(logits, *d.tensors())
-            ctx.d, ctx.world = d, world
+            ctx.d, ctx.world, ctx.captured = d, world, torch.cuda.is_current_stream_capturing()
         if world > 1:
             d.row_stats(logits)
             d.reduce(0, rows, group)
@@ -281,6 +292,7 @@ class _DistillFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
+        _captured_with_forward(ctx)
         dloss = dloss.to(torch.float32)
         early, ctx.early = ctx.early, None
         if early is not None and not torch.cuda.is_current_stream_capturing():
@@ -442,7 +454,8 @@ def _head_pass(hidden, weight, teacher, temperature, share, vocab_lo, group, chu
     count = torch.empty((T + chunk_rows - 1) // chunk_rows, device=dev, dtype=torch.int32)
     nv.call("mmt_compact_labels", need.data_ptr(), T, chunk_rows, src.data_ptr(), lab.data_ptr(), pos.data_ptr(),
             count.data_ptr(), nv.stream())
-    x = F.gather_rows_raw(hidden, src)
+    # `lab` is `src` less the rows without either inside a group that is kept: what they hold stays out of the products
+    x = F.gather_rows_raw(hidden, lab)
     dx = torch.empty_like(hidden) if need_h else None
     ws = torch.empty(chunk_rows, V, device=dev, dtype=torch.float32)
     gs = torch.empty(chunk_rows, V, device=dev, dtype=torch.bfloat16) if need_h or dw is not None else None
@@ -491,18 +504,17 @@ class _LMHeadDistillFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
+        _captured_with_forward(ctx)
         grads = ctx.grads
-        if ctx.captured or torch.cuda.is_current_stream_capturing():
-            if grads is None:
-                raise RuntimeError("a backward pass of lm_head_distillation is captured after an eager one")
-            grads = [None if g is None else g * dloss.to(g.dtype) for g in grads]
-            return (*grads,) + (None,) * (3 + len(ctx.call))
-        if grads is None:
+        if ctx.captured:
+            grads = [None if g is None else g.clone() for g in grads]
+        elif grads is None:
             hidden, weight, *teacher = ctx.saved_tensors
             need_h, need_w = ctx.need
             dw = torch.empty_like(weight) if need_w else None
             grads = (_head_pass(hidden, weight, teacher, *ctx.call, need_h, dw, False)[1], dw)
-        ctx.grads = None
+        if not ctx.captured:
+            ctx.grads = None
         dloss = dloss.to(torch.float32)
         for g in grads:
             if g is not None:
@@ -615,7 +627,8 @@ def _verify_reference(target, draft_ids, draft, uniforms, temperature, lens) -> 
             else:
                 qa = torch.zeros_like(w).scatter_(1, at[rows, spot][:, None], known[rows, spot].double()[:, None])
             rest = (w - qa).clamp(min=0.0)
-            w = torch.where((a < lens)[:, None] & (rest.sum(1, keepdim=True) > 0), rest, w)
+            least = 0.0 if q is None else 2.0 ** -46      # of p that is q but for its rounding
+            w = torch.where((a < lens)[:, None] & (rest.sum(1, keepdim=True) > least), rest, w)
         sums = w.cumsum(1)
         goal = u[:, n:] * sums[:, -1:]
         first = (sums <= goal).sum(1)
@@ -637,8 +650,8 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
     ``draft_logits`` [B, n, V] are what the drafts were drawn from; None: tokens that were looked up or chosen, all of
     whose probability counts as theirs.  ``uniforms`` [B, n + 1] (fp32 or fp64, in [0, 1)) are the random numbers: column i
     accepts draft i if ``u q(x) < p(x)`` with p, q = softmax(logits / temperature), the last column draws the next token
-    from ``max(p - q, 0)`` at the first rejected place (from p if that has no mass), or from the target's row behind the
-    last draft.  The tokens then have the target's own distribution.
+    from ``max(p - q, 0)`` at the first rejected place (from p if that has no mass beyond rounding), or from the target's
+    row behind the last draft.  The tokens then have the target's own distribution.
 
     ``temperature == 0``: greedy, without ``draft_logits`` and ``uniforms``: a draft stands while it is the id of the
     largest logit (lowest id among equals, NaN above everything), which is also the next token.

@@ -204,6 +204,94 @@ def test_distillation_of_rows_masked_with_the_lowest_value(dtype, temperature, s
     _near(*_loss_and_grad(x, ids, teacher, temperature=temperature, labels=labels, label_weight=share), *want, temperature, dtype)
 
 
+@pytest.mark.parametrize("dtype,V", [(BF16, 820_001), (F32, 410_003)])
+@pytest.mark.parametrize("temperature,share", [(2.0, 0.3), (1.0, 0.5)])
+def test_distillation_of_a_vocabulary_that_no_cluster_holds(dtype, V, temperature, share):
+    x, ids, teacher, labels = _batch(6, V, 5, dtype)
+    labels[2] = 7
+    x[4] = torch.finfo(dtype).min
+    want = oracle.distill(x, ids, teacher, temperature, labels, share)
+    _near(*_loss_and_grad(x, ids, teacher, temperature=temperature, labels=labels, label_weight=share), *want, temperature, dtype)
+
+
+@pytest.mark.parametrize("temperature,share", [(1.0, 0.0), (2.0, 0.3), (0.5, 1.0)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_distillation_of_vocabulary_shards(monkeypatch, dtype, temperature, share):
+    """The ranks are threads that meet on the host where they would reduce."""
+    import threading
+    from multimodal_training_b200.ops import vocab_rows
+    F = _ops()
+    T, V, K, world = 12, 1000, 6, 2
+    x, ids, teacher, labels = _batch(T, V, K, dtype)
+    x[4, :V // 2] = -INF                            # one shard has nothing
+    ids[4], labels[4] = torch.arange(V // 2, V // 2 + K, device="cuda"), V - 1
+    x[5, V // 2:], x[8] = torch.finfo(dtype).min, torch.finfo(dtype).min
+    ids[5], ids[8], labels[8] = torch.arange(K, device="cuda"), torch.arange(497, 497 + K, device="cuda"), 500
+    meet, given, rank_of = threading.Barrier(world, timeout=60), [None] * world, threading.local()
+
+    def all_reduce(t, op, group):
+        given[rank_of.rank] = t.clone()
+        meet.wait()
+        both = torch.stack(given)
+        meet.wait()
+        t.copy_(both.amax(0) if op == torch.distributed.ReduceOp.MAX else both.sum(0))
+
+    monkeypatch.setattr(F, "_all_reduce", all_reduce)
+    labels_or_none = None if share == 0 else labels
+    out = [None] * world
+
+    def rank(r):
+        rank_of.rank = r
+        lo = r * (V // world)
+        mine = x[:, lo:lo + V // world]
+        d = vocab_rows._Distill(ids, teacher, labels_or_none, temperature, share, lo, V, dtype == F32, V // world)
+        d.row_stats(mine)
+        d.reduce(0, T, None)
+        grad = torch.empty(T, V // world, device="cuda", dtype=dtype)
+        d.grad(mine, grad)
+        out[r] = d.loss(), grad
+
+    threads = [threading.Thread(target=rank, args=(r,)) for r in range(world)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert torch.equal(out[0][0], out[1][0])
+    _near(out[0][0], torch.cat([g for _, g in out], 1), *oracle.distill(x, ids, teacher, temperature, labels, share), temperature,
+          dtype)
+
+
+def test_rows_that_all_weight_leaves_are_not_read():
+    x, ids, teacher, labels = _batch(8, 500, 4, BF16)
+    labels[:] = torch.tensor([3, -100] * 4)
+    want = _loss_and_grad(x, ids, teacher, labels=labels, label_weight=1.0)
+    x[1::2] = NAN                                   # a teacher without weight, no label
+    got = _loss_and_grad(x, ids, teacher, labels=labels, label_weight=1.0)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and not got[1][1::2].any()
+
+
+def test_rows_of_a_broadcast_batch():
+    x, ids, teacher, _ = _batch(1, 3001, 5, BF16)
+    wide = x.detach().requires_grad_()
+    loss = _ops().distillation_loss(wide.expand(40, 3001).unflatten(0, (4, 10)), ids.expand(4, 10, 5), teacher.expand(4, 10, 5))
+    want, dx, size = oracle.distill(x, ids, teacher)
+    # a fortieth each, rounded, whose sum rounds to bf16 once more (or on the way: 40 terms at half a step each)
+    (grad,) = torch.autograd.grad(loss, wide)
+    assert ((grad.cpu().double() - dx).abs() <= 2.0 ** -8 * 41 * dx.abs() + 2.0 ** -15 * size + 1e-37).all()
+    assert abs(loss.item() - want) <= 2.0 ** -15
+    values, top = _ops().top_logits(x.expand(3, 3001), 4)
+    assert torch.equal(top, top[:1].expand(3, 4)) and torch.equal(top[:1].cpu(), oracle.top(x, 4)[1])
+
+
+def test_a_captured_backward_pass_has_a_captured_forward_pass(monkeypatch):
+    F = _ops()
+    x, ids, teacher, _ = _batch(4, 64, 4, BF16)
+    w = torch.ones(64, 64, device="cuda", dtype=BF16)
+    losses = F.distillation_loss(x.requires_grad_(), ids, teacher), F.lm_head_distillation(x, w, ids, teacher)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for loss in losses:
+        with pytest.raises(RuntimeError, match="capture both"):
+            loss.backward()
+
+
 def test_ids_outside_the_vocabulary_are_left_out_and_reported():
     from multimodal_training_b200.ops import native as nv
     x, ids, teacher, labels = _batch(8, 300, 6, BF16)
@@ -273,6 +361,42 @@ def test_head(T, H, V, K, chunk, temperature, share):
     assert torch.equal(only, got[1] * 2)
 
 
+def test_head_of_chunks_that_differ_in_size():
+    """A last chunk of 6 rows has more blocks for a row than the ones before, and the vocabulary of its gradient is cut."""
+    F = _ops()
+    T, H, V, K = 70, 64, 20000, 5
+    g = torch.Generator().manual_seed(1)
+    h = torch.randn(T, H, generator=g).cuda().bfloat16().requires_grad_()
+    w = (torch.randn(V, H, generator=g) / 8).cuda().bfloat16().requires_grad_()
+    _, ids, teacher, labels = _batch(T, V, K, BF16)
+    hd, wd = h.detach().double().cpu().requires_grad_(), w.detach().double().cpu().requires_grad_()
+    z = hd @ wd.T
+    want, dz, _ = oracle.distill(z, ids, teacher, 2.0, labels, 0.3)
+    dh, dw = torch.autograd.grad(z, (hd, wd), dz)
+    junk = [torch.full((n,), NAN, device="cuda", dtype=torch.float64) for n in (70, 140, 560) for _ in range(40)]
+    del junk                                        # what the workspaces hold before
+    loss = F.lm_head_distillation(h, w, ids, teacher, temperature=2.0, labels=labels, label_weight=0.3, chunk_rows=64)
+    # fp32 logits: sums of 64 products in fp32, 2^-18 of numbers of up to 5, times tau^2
+    assert abs(loss.item() - want) < 2.0 ** -12
+    for a, b in zip(torch.autograd.grad(loss, (h, w)), (dh, dw)):
+        assert (a.cpu().double() - b).norm() <= 8e-3 * b.norm()
+
+
+def test_head_of_hidden_states_that_are_not_numbers_where_nothing_is_taught():
+    F = _ops()
+    T, H, V, K = 80, 64, 520, 4
+    h = torch.randn(T, H, device="cuda").bfloat16()
+    w = torch.randn(V, H, device="cuda").bfloat16().requires_grad_()
+    _, ids, teacher, _ = _batch(T, V, K, BF16)      # every fourth row is without a teacher
+    want = torch.autograd.grad(F.lm_head_distillation(h.requires_grad_(), w, ids, teacher), (h, w))
+    h = h.detach().clone()
+    h[1::4] = NAN
+    h[5::8] = INF
+    got = torch.autograd.grad(F.lm_head_distillation(h.requires_grad_(), w, ids, teacher), (h, w))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
 def test_head_writes_into_the_flat_gradient():
     F = _ops()
     T, H, V, K = 90, 128, 520, 7
@@ -330,6 +454,24 @@ def test_verification(B, n, V, dtype, temperature, drafter):
             got = F.verify_drafts(_laid_out(target, lay), ids, None if draft is None else _laid_out(draft, lay), u,
                                   temperature=temperature, draft_lens=ln)
             _same(got, oracle.verify(target, ids, draft, u, temperature, ln))
+
+
+@pytest.mark.parametrize("B", [1, 20, 48, 200])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_more_drafts_than_a_warp_has_lanes(B, dtype, temperature):
+    F = _ops()
+    n, V = 70, 300
+    target, ids, draft, u = _drafts(B, n, V, dtype, seed=B)
+    draft[::2] = target[::2, :n]                    # such drafts stand, whatever the uniforms
+    if temperature == 0:
+        ids[::2] = target[::2, :n].float().argmax(-1)
+    ids[::2] = torch.where(torch.arange(n, device="cuda") < 20 + torch.arange(B, device="cuda")[::2, None] * 7 % 53, ids[::2], -1)
+    got = (F.verify_drafts(target, ids, draft, u, temperature=temperature) if temperature else
+           F.verify_drafts(target, ids, temperature=0.0))
+    _same(got, oracle.verify(target, ids, draft, u, temperature) if temperature else
+          oracle.verify(target, ids, None, None, 0.0))
+    assert got.accepted.max() >= 20
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -431,6 +573,61 @@ def test_another_stream():
     for a, b in zip(want, got):
         for p, q in zip(a, b):
             assert torch.equal(p, q)
+
+
+def test_two_streams_at_once():
+    F = _ops()
+    batches = [(_batch(40, 50001, 8, BF16, seed=s), _drafts(3, 3, 20001, BF16, seed=s)) for s in (0, 1)]
+
+    def work(b):
+        (x, ids, teacher, _), (target, dids, draft, u) = b
+        return (*F.top_logits(x, 5), *_loss_and_grad(x, ids, teacher), *F.verify_drafts(target, dids, draft, u))
+
+    want = [work(b) for b in batches]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in batches]
+    got = [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(work(batches[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for run in got[i]:
+            for a, b in zip(run, want[i]):
+                assert torch.equal(a, b)
+
+
+def test_teacher_student_and_draft_model_as_they_are_used():
+    """The same weights on both devices: top logits, the student's step and an answer with a draft model."""
+    from multimodal_training_b200.models.vlm import Qwen2_5_VLForConditionalGeneration as Model
+    from test_vlm_wrapper import _batch as sample
+    cpu = [Model("smoke", seed=s) for s in (3, 4)]
+    gpu = [Model("smoke", seed=s).cuda().bfloat16() for s in (3, 4)]
+    ids, pix, labels = sample(cpu[0].config, [(1, 16, 16)], text_len=24)
+    grid = [(1, 16, 16)]
+    losses = []
+    for teacher, student in (cpu, gpu):
+        dtype = student.model.language_model.embed_tokens.dtype
+        dev = student.model.language_model.embed_tokens.device
+        pix = pix.to(dtype)
+        values, top = teacher.top_logits(9, ids, pix, grid)
+        out = student(ids, pix, grid, labels=labels, teacher_ids=top, teacher_logits=values, temperature=2.0, label_weight=0.25)
+        out["loss"].backward()
+        losses.append(out["loss"].item())
+        assert all(p.grad.isfinite().all() for p in student.parameters() if p.grad is not None)
+        # what the operators say on this device of this device's logits
+        logits = teacher(ids, pix, grid)["logits"].detach()
+        assert torch.equal(logits.gather(1, top.clamp(min=0))[top[:, 0] >= 0], values[top[:, 0] >= 0])
+        plain = teacher.generate(ids[0], pix, grid, max_new_tokens=6)
+        with_draft = teacher.generate(ids[0], pix, grid, 6, draft_model=student, draft_tokens=3)
+        drawn = teacher.generate(ids[0], pix, grid, 6, temperature=0.8, draft_model=student, draft_tokens=3,
+                                 generator=torch.Generator(dev).manual_seed(0))
+        assert plain.shape == with_draft.shape == drawn.shape == (ids.numel() + 6,)
+        assert (drawn >= 0).all() and (drawn < teacher.config.text.vocab_size).all()
+        assert dtype == (F32 if dev.type == "cpu" else BF16)
+    # bf16 hidden states through a few layers: 2^-8 a rounding, a few tens of them, of logits of about one
+    assert abs(losses[0] - losses[1]) < 0.1 * abs(losses[0])
 
 
 def test_two_graphs_of_all_operators_replayed_in_turn():

@@ -69,3 +69,27 @@ def test_sampled_answers_and_refusals():
         draw(draft_model=draft, draft_tokens=0)
     with pytest.raises(ValueError):
         draw(draft_model=Qwen2_5_VLForConditionalGeneration("smoke", seed=6))
+
+
+def test_logits_that_are_no_distribution_are_refused():
+    target = Qwen2_5_VLForConditionalGeneration("tiny", seed=5)
+    draft = Qwen2_5_VLForConditionalGeneration("tiny", seed=6)
+    ids = torch.randint(0, 900, (5,), generator=torch.Generator().manual_seed(1))
+    with torch.no_grad():
+        draft.model.language_model.norm_w.fill_(float("nan"))
+    for model, kw in ((target, dict(draft_model=draft)), (draft, {})):
+        with pytest.raises(RuntimeError, match="no distribution"):
+            model.generate(ids, max_new_tokens=3, temperature=1.0, **kw)
+
+
+def test_placeholders_are_not_drawn():
+    m = Qwen2_5_VLForConditionalGeneration("tiny", seed=5)
+    ids = torch.randint(0, 900, (5,), generator=torch.Generator().manual_seed(1))
+    with torch.no_grad():                           # nothing but the two placeholders would be drawn
+        m.model.language_model.logits = lambda h, plain=m.model.language_model.logits: plain(h).index_add(
+            1, torch.tensor([m.config.image_token_id, m.config.video_token_id]), torch.full((h.shape[0], 2), 1e4))
+        got = m.generate(ids, max_new_tokens=6, temperature=1.0, generator=torch.Generator().manual_seed(0))
+    assert got.numel() == 11
+    assert not ((got == m.config.image_token_id) | (got == m.config.video_token_id)).any()
+    with pytest.raises(ValueError, match="negative"):
+        m.generate(ids, max_new_tokens=2, temperature=-1.0)
