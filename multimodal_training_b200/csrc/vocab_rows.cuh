@@ -80,8 +80,6 @@ struct Row {
     }
     return make_uint4((uint32_t)half[0], (uint32_t)(half[0] >> 32), (uint32_t)half[1], (uint32_t)(half[1] >> 32));
   }
-  // Writes the columns of vector i to the row `out`, of this type or a narrower one, whose start (`out_lead` elements behind
-  // a boundary of kVec of them) may lie otherwise.
   template <typename O>
   static MMT_DEVICE int lead_for(const O* out) { return (int)(reinterpret_cast<uintptr_t>(out) / sizeof(O) % kVec); }
   template <typename O>
@@ -89,6 +87,8 @@ struct Row {
     if constexpr (sizeof(O) == sizeof(T)) *reinterpret_cast<uint4*>(to) = RowVec<T>::pack(v);
     else *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
   }
+  // Writes the columns of vector i to the row `out`, of this type or a narrower one, whose start (`out_lead` elements behind
+  // a boundary of kVec of them) may lie otherwise.
   template <typename O>
   MMT_DEVICE void store(O* out, int out_lead, int i, const float (&v)[kVec]) const {
     const int c = column(i);

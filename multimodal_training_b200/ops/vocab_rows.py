@@ -176,27 +176,28 @@ class _Distill:
                  need: torch.Tensor | None = None):
         _same_layout("mmt_distill_bytes", ctypes.sizeof(_DistillWords))
         rows, K = teacher_ids.shape
-        dev = teacher_ids.device
-        per = nv.lib().mmt_distill_count_rows()
+        lib = nv.lib()
+        per, n_stats = lib.mmt_distill_count_rows(), lib.mmt_distill_stats_count()
         n_counts = (rows + per - 1) // per
-        self.stats = torch.empty(nv.lib().mmt_distill_stats_count(), rows, device=dev, dtype=torch.float64)
-        self.info = torch.empty(rows, 2, device=dev, dtype=torch.float64)
-        self.small = torch.empty(2 * rows * (K + 1) + rows + 2 * n_counts + 2, device=dev, dtype=torch.int32)
-        at = self.small.data_ptr()
+        # one workspace, 8-byte words first: statistics, info, pairs of counts, tickets, ids and probabilities, marks
+        n_slots = rows * (K + 1)
+        self.n_stats = n_stats * rows
+        at_counts = self.n_stats + 2 * rows
+        words = at_counts + n_counts + 1
+        self.work = torch.empty(words + n_slots + (rows + 1) // 2, device=teacher_ids.device, dtype=torch.float64)
+        at = self.work.data_ptr()
         w = self.words = _DistillWords(rows=rows, vocab_lo=vocab_lo, temperature=temperature, share=share, V=V, K=K,
-                                       is_f32=int(is_f32), info=self.info.data_ptr(), stats=self.stats.data_ptr())
-        w.counts = at                                        # pairs of counts first: 8 bytes each
-        w.slot_id = at + 8 * n_counts
-        w.slot_p = w.slot_id + 4 * rows * (K + 1)
-        w.mark = w.slot_p + 4 * rows * (K + 1)
-        w.ticket = w.mark + 4 * rows
+                                       is_f32=int(is_f32), stats=at, info=at + 8 * self.n_stats, counts=at + 8 * at_counts,
+                                       ticket=at + 8 * (words - 1), slot_id=at + 8 * words,
+                                       slot_p=at + 8 * words + 4 * n_slots, mark=at + 8 * (words + n_slots))
         if rows:
             nv.call("mmt_distill_prepare", ctypes.addressof(w), teacher_ids.data_ptr(), _ld(teacher_ids),
                     teacher_logits.data_ptr(), _ld(teacher_logits), int(teacher_logits.dtype == torch.float32),
                     nv.ptr(labels), vocab_total, nv.ptr(need), nv.stream())
 
-    def tensors(self) -> tuple[torch.Tensor, ...]:
-        return self.stats, self.info, self.small
+    @property
+    def stats(self) -> torch.Tensor:
+        return self.work[:self.n_stats].view(nv.lib().mmt_distill_stats_count(), self.words.rows)
 
     def _rows(self, logits, src, cnt):
         w = self.words
@@ -211,10 +212,11 @@ class _Distill:
     def reduce(self, lo: int, hi: int, group) -> None:
         """Statistics of rows [lo, hi) over the shards of the vocabulary."""
         from . import functional as F
-        top = self.stats[:2, lo:hi].contiguous()
+        stats = self.stats
+        top = stats[:2, lo:hi].contiguous()
         mine = top.clone()
         F._all_reduce(top, torch.distributed.ReduceOp.MAX, group)
-        rest = self.stats[2:, lo:hi].contiguous()
+        rest = stats[2:, lo:hi].contiguous()
         sums, label, dot, mass, has_label = rest[:2], rest[2], rest[3], rest[4], rest[5]
         # from below this shard's largest logit to below the whole vocabulary's; a shard of nothing but -inf has a sum of
         # zero, which stays
@@ -223,8 +225,8 @@ class _Distill:
         label.add_(torch.where(has_label > 0, down[1], 0.0))
         dot.add_(torch.where(mass > 0, mass * down[0], 0.0))
         F._all_reduce(rest, torch.distributed.ReduceOp.SUM, group)
-        self.stats[:2, lo:hi] = top
-        self.stats[2:, lo:hi] = rest
+        stats[:2, lo:hi] = top
+        stats[2:, lo:hi] = rest
 
     def _out(self, out, dloss=None) -> None:
         w = self.words
@@ -252,7 +254,7 @@ class _Distill:
             nv.call("mmt_distill_grad", ctypes.addressof(w), nv.stream())
 
     def loss(self) -> torch.Tensor:
-        out = torch.empty((), device=self.stats.device, dtype=torch.float32)
+        out = torch.empty((), device=self.work.device, dtype=torch.float32)
         nv.call("mmt_distill_loss", ctypes.addressof(self.words), out.data_ptr(), nv.stream())
         return out
 
@@ -278,7 +280,7 @@ class _DistillFn(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             if not torch.cuda.is_current_stream_capturing():
                 ctx.early = torch.empty(rows, V, device=logits.device, dtype=logits.dtype)
-            ctx.save_for_backward(logits, *d.tensors())
+            ctx.save_for_backward(logits, d.work)
             ctx.d, ctx.world, ctx.captured = d, world, torch.cuda.is_current_stream_capturing()
         if world > 1:
             d.row_stats(logits)
