@@ -12,6 +12,8 @@
 // S = sum 2^((x - m) c).  Statistics and gradient use the same rounded c, which changes the temperature by 2^-24 and nothing
 // else; the difference is taken first, so any finite logits do, the lowest of their type among them.  S is summed in fp32
 // (relative error of a few 2^-24); everything that is K long is fp64.
+#include <numeric>
+
 #include "vocab_rows.cuh"
 
 namespace {
@@ -335,24 +337,29 @@ __global__ void __launch_bounds__(kDistillThreads) distill_grad_kernel(const T* 
 // that into every CTA of the cluster, and behind one cluster barrier all of them know the row's statistics.  A logit is read
 // once and its gradient written once.
 //
-// Second softmax (kMode): none, or that of temperature one for the labels.  If the temperature is a power of two, its powers
-// are the first one's squared log2(tau) times (c1 = tau c exactly).
+// Second softmax (kMode): none, or that of temperature one for the labels.  If the temperature is two or four, its powers are
+// the first one's squared once or twice (c1 = tau c exactly): 200 us instead of 233 for the case of launch_mode.
 //
 // The parts travel as asynchronous stores that count themselves into an mbarrier of the CTA they go to (two of them, in
 // turn: a CTA may be a row ahead of another, never two).  A barrier of the cluster would also wait until the gradients that
 // the threads have stored are visible, which is several microseconds.
 //
+// What bounds it is issue (46 % of the cycles) and the chain of a row, copy to exchange to gradient, more than memory (53 %);
+// so the rows are visited in an order that mixes neighbours: those without a teacher, which are only cleared, come in long runs
+// (image tokens), and their stores run beside the others' arithmetic this way.  The case of launch_mode: 234 us in order, 216
+// mixed, both before the second powers' squarings were unrolled; with 256 threads instead of 128, 242 and 232.
+//
 // Rows are handed out by tickets: a cluster knows its row and the next one, whose copy starts as soon as the row's gradients
 // are formed, and takes a ticket for the one after that, which travels with the parts.
 // ----------------------------------------------------------------------------
-constexpr int kSingle = 0, kSquares = 1, kTwice = 2;
+constexpr int kSingle = 0, kTwice = -1;            // or the number of squares
+constexpr int kFewThreads = 128;                   // of a CTA that holds a short run
 
 // The two powers of two logits below `m`, with c = (c, c) and so on.
 struct Powers {
   f32x2 c, c1, less;
-  int squares;
-  MMT_DEVICE Powers(const DistillCall& call, float m, int squares_)
-      : c(both(call.c, call.c)), c1(both(call.c1, call.c1)), less(both(-m, -m)), squares(squares_) {}
+  MMT_DEVICE Powers(const DistillCall& call, float m)
+      : c(both(call.c, call.c)), c1(both(call.c1, call.c1)), less(both(-m, -m)) {}
   template <int kMode>
   MMT_DEVICE void take(f32x2 x, f32x2& e, f32x2& e1) const {
     x = add2(x, less);
@@ -362,20 +369,21 @@ struct Powers {
       v = apart(mul2(x, c1));
       e1 = both(pow2(v.x), pow2(v.y));
     }
-    if constexpr (kMode == kSquares) {
+    if constexpr (kMode > 0) {
       e1 = mul2(e, e);
-      for (int k = 1; k < squares; ++k) e1 = mul2(e1, e1);
+#pragma unroll
+      for (int k = 1; k < kMode; ++k) e1 = mul2(e1, e1);
     }
   }
 };
 
 template <typename T, typename O, int kThreads, int kMode>
-__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
-    distill_fused_kernel(const T* logits, long ld, int V, DistillRows rows, DistillCall call, int squares, long n_rows,
-                         int places, const long* src, const int* cnt, double* __restrict__ stats, int* ticket,
-                         const float* dloss, O* out, long out_ld, int per, MmtErrorWord* ew) {
+__global__ void __launch_bounds__(kThreads, kThreads == kFewThreads ? 6 : 2)
+    distill_fused_kernel(const T* logits, long ld, int V, DistillRows rows, DistillCall call, long n_rows,
+                         int places, int step, const long* src, const int* cnt, double* __restrict__ stats,
+                         int* ticket, const float* dloss, O* out, long out_ld, int per, MmtErrorWord* ew) {
   grid_dependency_sync();
-  constexpr int kVec = Row<T>::kVec, kWarps = kThreads / 32;
+  constexpr int kVec = Row<T>::kVec, kWarps = kThreads / 32, kFix = (kMaxTop + kThreads) / kThreads;
   constexpr bool kDual = kMode != kSingle;
   extern __shared__ __align__(128) uint4 held[];   // this CTA's vectors of the row, `per` of them
   __shared__ uint64_t arrived, met[2];
@@ -421,7 +429,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
                  : "memory");
   };
   cluster_barrier();                               // every CTA has started: its shared memory may be written
-  int place = blockIdx.x / C, next = place + clusters;
+  // the q-th row that is handed out
+  auto place_of = [&](int q) { return q >= end ? end : step == 1 ? q : (int)((long)q * step % end); };
+  int place = place_of(blockIdx.x / C), next = place_of(blockIdx.x / C + clusters);
   int at = place < end ? row_at(place) : -1, mark = mark_of(at);
   if (tid == 0 && mark != 0) fetch(place);
   const int K1 = rows.K + 1;
@@ -440,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
   for (int k = 0; place < end; ++k) {
     const int turn = k & 1;
     int after = 0;
-    if (rank == 0 && warp == 0) after = 2 * clusters + (lane == 0 ? atomicAdd(ticket, 1) : 0);
+    if (rank == 0 && warp == 0 && lane == 0) after = place_of(2 * clusters + atomicAdd(ticket, 1));
     const Row<T> row = row_of(place);
     const int n = max(min(per, row.vectors() - first), 0);
     const int2 mid = whole(row, n);
@@ -466,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       // a warp that has nothing but -inf adds zeros (2^-inf), not 2^(-inf + inf)
       f32x2 s2 = both(0.f, 0.f), s12 = s2;
       {
-        const Powers pw(call, m == -INFINITY ? 0.f : m, squares);
+        const Powers pw(call, m == -INFINITY ? 0.f : m);
 #pragma unroll 2
         for (int i = tid; i < n; i += kThreads) {
           float v[kVec];
@@ -524,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       const int label_at = mark & kLabelled ? mark >> kSlotShift : -1;
       const float wt = mark & kTaught ? w_taught : 0.f, wl = mark & kLabelled ? w_labelled : 0.f;
       const float a = (kDual ? wt : wt + wl) / S, a1 = kDual ? wl / S1 : 0.f;
-      const Powers pw(call, top, squares);
+      const Powers pw(call, top);
       const f32x2 a2 = both(a, a), a12 = both(a1, a1);
       auto grad = [&](float x, float y) {
         f32x2 e, e1;
@@ -557,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
           row.store(o, o_lead, first + i, v);
         }
       }
-      // the slots that this CTA holds: their gradients (two slots a thread at most), and one warp's part of the row's loss
+      // the slots that this CTA holds: their gradients (kFix slots a thread at most), and one warp's part of the row's loss
       auto held_slot = [&](int j, int& id, float& p, float& x) {
         id = j < K1 ? slot_ids[turn][j] : -1;
         if (id < 0 || (unsigned)((id + row.lead) / kVec - first) >= (unsigned)n) return false;
@@ -566,11 +576,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
         return true;
       };
       int id;
-      float p, x, fix[2];
-      int fix_at[2] = {-1, -1};
+      float p, x, fix[kFix];
+      int fix_at[kFix];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < kFix; ++b) {
         const int j = tid + b * kThreads;
+        fix_at[b] = -1;
         if (!held_slot(j, id, p, x)) continue;
         fix_at[b] = id;
         fix[b] = grad(x, x).x - wt * p - (j == label_at ? wl : 0.f);
@@ -588,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
       if (tid == 0 && next_mark != 0) fetch(next);
       if (o) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < kFix; ++b)
           if (fix_at[b] >= 0) from_float(fix[b], o + fix_at[b]);
       }
       if (warp == kWarps - 1) {
@@ -755,10 +766,17 @@ long row_vectors(const MmtDistill& d) {
   return (d.V + vec - 2) / vec + 1;
 }
 
-constexpr int kHeldBytes = 40 * 1024, kMaxHeldBytes = 200 * 1024;
+// A step through n rows that visits them all, each far from the one before.
+int mixing_step(int n) {
+  int s = (int)(0.618 * n);
+  while (s > 1 && std::gcd(s, n) != 1) --s;
+  return s < 1 ? 1 : s;
+}
+
+constexpr int kHeldBytes = 39 * 1024, kMaxHeldBytes = 200 * 1024;
 
 template <typename T, typename O, int kThreads, int kMode>
-int launch_held(MmtDistill& d, int C, int per, int squares, void* stream) {
+int launch_held(MmtDistill& d, int C, int per, void* stream) {
   d.parts = max(d.parts, C);                // chunks of a batch differ in it
   auto kernel = distill_fused_kernel<T, O, kThreads, kMode>;
   static int allowed = 0;
@@ -775,28 +793,32 @@ int launch_held(MmtDistill& d, int C, int per, int squares, void* stream) {
     known_bytes = bytes;
   }
   const long clusters = d.places < most ? d.places : most;
+  const int step = d.cnt ? 1 : mixing_step((int)d.places);
   return (int)launch_cluster(kernel, (unsigned)(clusters * C), kThreads, C, bytes, VR_STREAM(stream),
-                             reinterpret_cast<const T*>(d.logits), d.ld, d.V, rows_of(d), call_of(d), squares, d.rows,
-                             (int)d.places, d.src, d.cnt, d.stats, d.ticket, d.dloss, reinterpret_cast<O*>(d.out), d.out_ld,
+                             reinterpret_cast<const T*>(d.logits), d.ld, d.V, rows_of(d), call_of(d), d.rows,
+                             (int)d.places, step, d.src, d.cnt, d.stats, d.ticket, d.dloss, reinterpret_cast<O*>(d.out), d.out_ld,
                              per, mmt_error_word());
 }
 template <typename T, typename O, int kMode>
-int launch_mode(MmtDistill& d, int squares, void* stream) {
+int launch_mode(MmtDistill& d, void* stream) {
   const long nv = row_vectors(d);
-  // as few CTAs a row as hold it in 40 KB each, of which an SM has four; more where there are few rows
+  // As few CTAs a row as hold it in 39 KB each, of which an SM has five (smaller runs: six); more where there are few rows.
+  // 2048 x 152064 bf16, half of the rows with a teacher, two softmaxes: 200 us in runs of 37 KB, 215 in runs of 75 KB with two
+  // CTAs an SM.  512 x 152064 fp32, which eight CTAs hold in 75 KB each: 108 us
+  // with 256 threads, 110 with 512.
   int C = 1;
   while (C < kMaxCluster && nv * 16 > (long)kHeldBytes * C) C *= 2;
   while (C < kMaxCluster && d.places * C * 2 <= 2 * mmt_sm_count() && nv > 512L * C) C *= 2;
   const int per = (int)((nv + C - 1) / C);
-  return per * 16 <= kHeldBytes ? launch_held<T, O, 256, kMode>(d, C, per, squares, stream)
-                                : launch_held<T, O, 512, kMode>(d, C, per, squares, stream);
+  return per * 16 <= kHeldBytes ? launch_held<T, O, kFewThreads, kMode>(d, C, per, stream)
+                                : launch_held<T, O, 256, kMode>(d, C, per, stream);
 }
 template <typename T, typename O>
 int launch_fused(MmtDistill& d, void* stream) {
-  if (!dual(d)) return launch_mode<T, O, kSingle>(d, 0, stream);
-  if (d.temperature == 2.0 || d.temperature == 4.0 || d.temperature == 8.0)
-    return launch_mode<T, O, kSquares>(d, d.temperature == 2.0 ? 1 : d.temperature == 4.0 ? 2 : 3, stream);
-  return launch_mode<T, O, kTwice>(d, 0, stream);
+  if (!dual(d)) return launch_mode<T, O, kSingle>(d, stream);
+  if (d.temperature == 2.0) return launch_mode<T, O, 1>(d, stream);
+  if (d.temperature == 4.0) return launch_mode<T, O, 2>(d, stream);
+  return launch_mode<T, O, kTwice>(d, stream);
 }
 
 }  // namespace
