@@ -4,12 +4,13 @@
 // torch.topk has it; -0 equal to +0) above the inverted column, so that keys are unique and equal logits go by the lower
 // column.  The answer is the k largest keys of the row.
 //
-// One pass over the row, bound by memory: what is left of the logits is the vectors of which an element reaches a lower bound of
-// the k-th largest.  The bound is the k-th largest of what the threads have seen as their two sets' largest, which are k different elements;
-// it is raised behind stretches 1, 2, 4, ... of the row, and a row in no special order leaves about k (1 + 1 + 1/2 + ...)
-// vectors.  Between those the warps do not wait for one another.  In the end the elements of these vectors that reach the last
-// bound, little more than k, are ranked by counting.  (Looking at the elements where a vector reaches the bound took as long as
-// the pass itself, 107 -> 226 us for 2048 x 152064 bf16 and k = 64: some lane of every third warp's load has one.)
+// One pass over the row, bound by memory (2048 x 152064 bf16, k = 64: 121 us, 5.1 TB/s).  What is left of the logits is the
+// vectors of which an element reaches a lower bound of the k-th largest.  The bound is the k-th largest of what the threads have
+// seen as their two sets' largest, which are k different elements; it is raised behind stretches 1, 2, 4, ... of the row, and a
+// row in no special order leaves about k (1 + 1 + 1/2 + ...) vectors.  Between those the warps do not wait for one another.  In
+// the end the elements of these vectors that reach the last bound, little more than k, are ranked.  (Looking at the elements
+// where a vector reaches the bound took as long as the pass itself, 107 -> 226 us for 2048 x 152064 bf16 and k = 64: some lane of
+// every third warp's load has one.)  Short rows and large k are bound by the chain of barriers of the bounds and of the ranking.
 //
 // Where there are too many of them (rising logits, many equal ones) the run is looked at once more, step by step, and the list
 // of candidates is cut to its k largest as soon as it fills up; the last of them is the next bound, and columns only grow, so
@@ -38,7 +39,7 @@ struct alignas(16) TopShared {
   int vec_at[kVecs];
   alignas(16) u64 list[kList + kTopEdge];
   u64 best[kTopMax];
-  int hist[kTopBins];
+  int hist[kTopBins], start[kTopBins];
   int digit, need, count;               // of find_digit
   int vecs, taken, kept;
   uint32_t warp_value[2][32];
@@ -150,17 +151,54 @@ MMT_DEVICE void rank_list(TopShared<kTopThreads>& s, int n, int k, int shift, ui
     }
     n = s.kept;
   }
-  if (tid == 0) s.list[n] = 0;                    // for the last pair
-  __syncthreads();
-  for (int i = tid; i < n; i += kTopThreads) {
-    const u64 key = s.list[i];
-    int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; j += 2) {
-      const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&s.list[j]);
-      rank += (v.x > key) + (v.y > key);
+  // At most k + 64 keys are left.  They go into 256 bins of their values, and a key's rank is what lies in the bins above plus
+  // the larger ones of its own bin.  (4096 x 2000 fp32 and k = 256: 61 us; 103 when the larger ones of all were counted.)
+  constexpr int kEach = (kTopMax + 64 + kTopThreads - 1) / kTopThreads;
+  u64 key[kEach];
+  uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    key[e] = tid + e * kTopThreads < n ? s.list[tid + e * kTopThreads] : 0;
+    if (key[e] != 0) {
+      lo = min(lo, (uint32_t)(key[e] >> 32));
+      hi = max(hi, (uint32_t)(key[e] >> 32));
     }
-    if (rank < k) out(rank, key);
+  }
+  for (int b = tid; b < kTopBins; b += kTopThreads) s.hist[b] = 0;
+  const uint2 range = range_of_block<kTopThreads>(s, lo, hi);
+  const int wide = range.y < range.x ? 0 : 32 - __clz((range.y - range.x) / kTopBins);
+  int bin[kEach], at[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    bin[e] = key[e] != 0 ? (int)(((uint32_t)(key[e] >> 32) - range.x) >> wide) : -1;
+    if (bin[e] >= 0) at[e] = atomicAdd(&s.hist[bin[e]], 1);
+  }
+  __syncthreads();
+  if (tid < 32) {                                 // where the bins' keys start, from the last bin down
+    constexpr int kLane = kTopBins / 32;
+    const int from = kTopBins - 1 - kLane * tid;
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) mine += s.hist[from - j];
+    int before = up_to_lane(mine) - mine;
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) {
+      s.start[from - j] = before;
+      before += s.hist[from - j];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kEach; ++e)
+    if (bin[e] >= 0) s.list[s.start[bin[e]] + at[e]] = key[e];
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    if (bin[e] < 0) continue;
+    int rank = s.start[bin[e]];
+    const int end = rank + s.hist[bin[e]];
+    for (int j = rank; j < end; ++j) rank += s.list[j] > key[e];
+    if (rank < k) out(rank, key[e]);
   }
   __syncthreads();
 }
@@ -336,11 +374,13 @@ int launch_top(const void* logits, void* values, long* ids, long rows, int V, lo
   while (C < kTopCluster && rows * C * 2 <= 2L * mmt_sm_count() && nv > 512L * C) C *= 2;
   const int per = (int)((nv + C - 1) / C);
   // Short rows have few stretches, and more of them fit an SM in smaller CTAs; a large k needs many values for its bound.
-  // 4096 x 5000 bf16, k = 64: 34 us with 128 threads, 43 with 256, 62 with 512; 4096 x 2000 fp32, k = 256: 111, 105, 123;
-  // 1024 x 152064 bf16, k = 256: 486, 196, 94.
-  if (per <= 2048 && C == 1 && k <= 64) return launch_threads<T, 128>(logits, values, ids, rows, V, ld, k, vocab_lo, C, per, stream);
-  return per <= 4096 && C == 1 ? launch_threads<T, 256>(logits, values, ids, rows, V, ld, k, vocab_lo, C, per, stream)
-                               : launch_threads<T, 512>(logits, values, ids, rows, V, ld, k, vocab_lo, C, per, stream);
+  // us with 128, 256 and 512 threads, 4096 rows in bf16: 5000 columns 33, 42, 60 (k = 64) and 97, 72, 88 (k = 256); 16000 columns
+  // 48, 57, 64 (k = 32) and 248, 101, 87 (k = 256); 2048 x 50000 and k = 32: 56, 54, 63; 1024 x 152064 and k = 256: 424, 172, 83.
+  if (C == 1 && k <= 64 && per <= 2048)
+    return launch_threads<T, 128>(logits, values, ids, rows, V, ld, k, vocab_lo, C, per, stream);
+  return C == 1 && per <= (k <= 64 ? 8192 : 1024)
+             ? launch_threads<T, 256>(logits, values, ids, rows, V, ld, k, vocab_lo, C, per, stream)
+             : launch_threads<T, 512>(logits, values, ids, rows, V, ld, k, vocab_lo, C, per, stream);
 }
 
 }  // namespace
