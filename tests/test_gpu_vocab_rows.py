@@ -78,6 +78,21 @@ def test_top_logits_of_many_rows(T):
     assert torch.equal(ids.cpu(), want_i) and torch.equal(values.cpu(), want_v)
 
 
+@pytest.mark.parametrize("V", [700, 3001, 30001, 70001])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kind", ["normal", "equal", "few", "rising", "special"])
+def test_top_logits_of_a_block_a_row(V, dtype, kind):
+    """So many rows that none is cut over blocks: the blocks of all sizes, also with ties and lists that overflow."""
+    F = _ops()
+    x = _rows_of(kind, 3, V, dtype)
+    for k in (8, 64, 65, 256):
+        values, ids = F.top_logits(x.repeat(100, 1), k)
+        want_v, want_i = oracle.top(x, k)
+        assert torch.equal(ids.cpu(), want_i.repeat(100, 1)), k
+        assert torch.equal(values.cpu().view(torch.int16 if dtype == BF16 else torch.int32),
+                           want_v.repeat(100, 1).view(torch.int16 if dtype == BF16 else torch.int32))
+
+
 def test_rows_behind_two_to_the_31_elements():
     F = _ops()
     ld, V = 1_100_000_003, 1001
