@@ -17,7 +17,7 @@ namespace {
 
 constexpr int kRowThreads = 256;                  // of a CTA that reads a part of a row
 constexpr int kRowAhead = 4;                      // vectors that a thread loads before it works on them
-constexpr int kDrawThreads = 512;
+constexpr int kDrawThreads = 256;
 constexpr int kDrawWarps = kDrawThreads / 32;
 constexpr int kDrawCluster = 16;                  // most CTAs that weigh a row
 constexpr double kLog2e = 1.44269504088896340736;
@@ -508,17 +508,21 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(Verify v) 
     }
     const uint32_t past = __ballot_sync(0xffffffffu, up_to > rest && x > kNothing);
     if (past) {
-      if (lane != __ffs(past) - 1) return;
-      double sum = up_to - x;
-      int chosen = -1;
-      for (int j = 0; j < Row<T>::kVec && !(chosen >= 0 && sum > rest); ++j) {
-        const int col = w.p.column(i0 + lane) + j;
-        const double y = col >= 0 && col < v.V ? w.of(w.p.p[col], col) : 0.0;
-        if (!(y > kNothing)) continue;
-        chosen = col;
-        sum += y;
+      // this vector: a lane weighs a column
+      const int who = __ffs(past) - 1;
+      const double before = __shfl_sync(0xffffffffu, up_to - x, who);
+      const int col = w.p.column(i0 + who) + lane;
+      const double y = lane < Row<T>::kVec && col >= 0 && col < v.V ? w.of(w.p.p[col], col) : 0.0;
+      double sum = y;
+#pragma unroll
+      for (int o = 1; o < Row<T>::kVec; o <<= 1) {
+        const double z = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += z;
       }
-      *token = chosen;
+      const uint32_t weighty = __ballot_sync(0xffffffffu, y > kNothing);
+      const uint32_t chosen = __ballot_sync(0xffffffffu, y > kNothing && before + sum > rest);
+      // by rounding the goal may lie behind the vector: its last column with any weight
+      if (lane == (chosen ? __ffs(chosen) - 1 : 31 - __clz(weighty | 1u))) *token = max(col, 0);
       return;
     }
     rest -= __shfl_sync(0xffffffffu, up_to, 31);
