@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 from typing import NamedTuple
 
 import torch
@@ -95,6 +96,7 @@ nv.declare("mmt_top_logits", nv.c_int, [nv._P, nv.c_int, nv._P, nv._P, nv.c_long
                                         nv._P])
 
 
+@torch.no_grad()
 def _top_reference(logits: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor]:
     values, ids = torch.sort(logits, dim=1, descending=True, stable=True)
     return values[:, :k].contiguous(), ids[:, :k].contiguous()
@@ -113,7 +115,6 @@ def _top_rows(logits: torch.Tensor, k: int, vocab_lo: int) -> tuple[torch.Tensor
     return values, ids
 
 
-@torch.no_grad()
 def top_logits(logits: torch.Tensor, k: int, *, vocab_lo: int = 0, group=None) -> tuple[torch.Tensor, torch.Tensor]:
     """The ``k`` largest logits of every row of [..., V], largest first, and their ids: ``(values, ids)``, both [..., k].
 
@@ -136,7 +137,7 @@ def top_logits(logits: torch.Tensor, k: int, *, vocab_lo: int = 0, group=None) -
         torch.distributed.all_gather(parts_i, ids, group=group)
         values, at = _top_rows(torch.cat(parts_v, 1), k, 0)
         ids = torch.cat(parts_i, 1).gather(1, at)
-    return values.view(*lead, k), ids.view(*lead, k)
+    return (values, ids) if logits.dim() == 2 else (values.view(*lead, k), ids.view(*lead, k))
 
 
 # --------------------------------------------------------------------------------------
@@ -412,7 +413,7 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     gpu = _on_gpu(logits, teacher_ids, teacher_logits, labels)
     ids, teacher, labels = _check_distill(logits.shape[:-1], logits.device, teacher_ids, teacher_logits, temperature, labels,
                                           label_weight)
-    rows = logits.reshape(-1, V)
+    rows = logits if logits.dim() == 2 else logits.reshape(-1, V)
     if not gpu:
         return _distill_reference(rows, ids, teacher, labels, temperature, label_weight, vocab_lo, group)
     return _DistillFn.apply(_rows(rows), ids, teacher, labels, float(temperature), float(label_weight), vocab_lo, group)
@@ -565,14 +566,7 @@ class Verified(NamedTuple):
     accept_prob: torch.Tensor    # [B, n] fp32: min(1, p / q) of every drafted token, 0 behind a sequence's last
 
 
-class _VerifyWords(ctypes.Structure):
-    _fields_ = [("target", ctypes.c_void_p), ("draft", ctypes.c_void_p), ("target_seq", ctypes.c_long),
-                ("target_row", ctypes.c_long), ("draft_seq", ctypes.c_long), ("draft_row", ctypes.c_long),
-                ("draft_ids", ctypes.c_void_p), ("uniforms", ctypes.c_void_p), ("lens", ctypes.c_void_p),
-                ("accepted", ctypes.c_void_p), ("tokens", ctypes.c_void_p), ("accept_prob", ctypes.c_void_p),
-                ("parts", ctypes.c_void_p), ("inv_temperature", ctypes.c_double), ("batch", ctypes.c_int),
-                ("drafts", ctypes.c_int), ("V", ctypes.c_int), ("is_f32", ctypes.c_int), ("uniforms_f64", ctypes.c_int),
-                ("sampled", ctypes.c_int), ("rows", ctypes.c_int), ("splits", ctypes.c_int)]
+_VERIFY_WORDS = struct.Struct("@2P4l7Pd8i")
 
 
 nv.declare("mmt_verify_bytes", nv.c_int, [])
@@ -580,6 +574,7 @@ nv.declare("mmt_verify_splits", nv.c_int, [nv.c_long, nv.c_int, nv.c_int])
 nv.declare("mmt_verify_drafts", nv.c_int, [nv._P, nv._P])
 
 
+@torch.no_grad()
 def _verify_reference(target, draft_ids, draft, uniforms, temperature, lens) -> Verified:
     """Plain PyTorch, in fp64."""
     B, m, V = target.shape
@@ -640,7 +635,6 @@ def _verify_reference(target, draft_ids, draft, uniforms, temperature, lens) -> 
     return finish(u[:, :n] * qx < px, ratio, draw)
 
 
-@torch.no_grad()
 def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_logits: torch.Tensor | None = None,
                   uniforms: torch.Tensor | None = None, *, temperature: float = 1.0,
                   draft_lens: torch.Tensor | None = None) -> Verified:
@@ -697,7 +691,7 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
     if not gpu:
         lens = torch.full((B,), n, dtype=torch.int64) if lens is None else lens.clamp(0, n)
         return _verify_reference(target_logits, draft_ids, draft_logits, uniforms, temperature, lens)
-    _same_layout("mmt_verify_bytes", ctypes.sizeof(_VerifyWords))
+    _same_layout("mmt_verify_bytes", _VERIFY_WORDS.size)
     dev = target_logits.device
     target = target_logits if target_logits.stride(2) == 1 or V == 1 else target_logits.contiguous()
     draft = draft_logits
@@ -713,15 +707,13 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
         rows, is_f32 = n + 1 + (n if draft is not None else 0), int(target.dtype == torch.float32)
         splits = nv.lib().mmt_verify_splits(B * rows, V, is_f32)
         parts = torch.empty(B * rows * splits, device=dev, dtype=torch.int64)
-        w = _VerifyWords(target=target.data_ptr(), draft=nv.ptr(draft), target_seq=target.stride(0),
-                         target_row=target.stride(1), draft_seq=draft.stride(0) if draft is not None else 0,
-                         draft_row=draft.stride(1) if draft is not None else 0, draft_ids=draft_ids.data_ptr(),
-                         uniforms=nv.ptr(uniforms), lens=nv.ptr(lens), accepted=accepted.data_ptr(),
-                         tokens=tokens.data_ptr(), accept_prob=prob.data_ptr(), parts=parts.data_ptr(),
-                         inv_temperature=1.0 / temperature if temperature else 0.0, batch=B, drafts=n, V=V,
-                         is_f32=is_f32, rows=rows, splits=splits,
-                         uniforms_f64=int(uniforms is not None and uniforms.dtype == torch.float64),
-                         sampled=int(temperature > 0.0))
-        nv.call("mmt_verify_drafts", ctypes.addressof(w), nv.stream())
+        # the words of the call in the order of Verify in csrc/verify.cu; a packed string costs a fifth of a ctypes structure
+        words = _VERIFY_WORDS.pack(
+            target.data_ptr(), 0 if draft is None else draft.data_ptr(), target.stride(0), target.stride(1),
+            0 if draft is None else draft.stride(0), 0 if draft is None else draft.stride(1), draft_ids.data_ptr(),
+            0 if uniforms is None else uniforms.data_ptr(), 0 if lens is None else lens.data_ptr(), accepted.data_ptr(),
+            tokens.data_ptr(), prob.data_ptr(), parts.data_ptr(), 1.0 / temperature if temperature else 0.0, B, n, V, is_f32,
+            int(uniforms is not None and uniforms.dtype == torch.float64), int(temperature > 0.0), rows, splits)
+        nv.call("mmt_verify_drafts", words, nv.stream())
         nv.launch_count += 1                       # rows, then sequences
     return Verified(accepted, tokens, prob)
