@@ -747,8 +747,9 @@ DistillCall call_of(const MmtDistill& d) {
   return {(float)(kLog2e / d.temperature), (float)kLog2e, (float)d.temperature, (float)d.share};
 }
 bool dual(const MmtDistill& d) { return d.share > 0.0 && d.temperature != 1.0; }
+constexpr long kMostRows = 0x7fff0000L;            // tickets are a few thousand more, and ints
 bool wrong(const MmtDistill& d) {
-  return d.K < 1 || d.K > kMaxTop || d.V < 1 || d.rows < 0 || d.places < 0 || d.rows > 0x7fffffffL || d.places > 0x7fffffffL;
+  return d.K < 1 || d.K > kMaxTop || d.V < 1 || d.rows < 0 || d.places < 0 || d.rows > kMostRows || d.places > kMostRows;
 }
 
 template <typename T, bool kDual>
