@@ -412,6 +412,27 @@ def test_head_of_hidden_states_that_are_not_numbers_where_nothing_is_taught():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("temperature,share", [(1.0, 0.0), (4.0, 0.5), (0.5, 1.0)])
+def test_losses_without_gradients(temperature, share):
+    F = _ops()
+    T, H, V, K = 37, 64, 1032, 6
+    x, ids, teacher, labels = _batch(T, V, K, F32)
+    kw = dict(temperature=temperature, labels=labels, label_weight=share)
+    want, _ = _loss_and_grad(x, ids, teacher, **kw)
+    with torch.no_grad():
+        assert torch.equal(F.distillation_loss(x.requires_grad_(), ids, teacher, **kw), want)
+    h = torch.randn(T, H, device="cuda").bfloat16().requires_grad_()
+    w = (torch.randn(V, H, device="cuda") / 8).bfloat16().requires_grad_()
+    want = F.lm_head_distillation(h, w, ids, teacher, **kw)
+    with torch.no_grad():
+        got = F.lm_head_distillation(h, w, ids, teacher, **kw)
+    assert torch.equal(got, want.detach()) and not got.requires_grad
+    # weight or hidden states alone
+    both = torch.autograd.grad(want, (h, w))
+    assert torch.equal(torch.autograd.grad(F.lm_head_distillation(h, w.detach(), ids, teacher, **kw), h)[0], both[0])
+    assert torch.equal(torch.autograd.grad(F.lm_head_distillation(h.detach(), w, ids, teacher, **kw), w)[0], both[1])
+
+
 def test_head_writes_into_the_flat_gradient():
     F = _ops()
     T, H, V, K = 90, 128, 520, 7
@@ -487,6 +508,15 @@ def test_more_drafts_than_a_warp_has_lanes(B, dtype, temperature):
     _same(got, oracle.verify(target, ids, draft, u, temperature) if temperature else
           oracle.verify(target, ids, None, None, 0.0))
     assert got.accepted.max() >= 20
+
+
+@pytest.mark.parametrize("drafter", [False, True])
+def test_a_large_batch_of_short_rows(drafter):
+    F = _ops()
+    target, ids, draft, u = _drafts(3000, 2, 37, F32)
+    draft = draft if drafter else None
+    _same(F.verify_drafts(target, ids, draft, u.double(), temperature=1.4),
+          oracle.verify(target, ids, draft, u, 1.4))
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
