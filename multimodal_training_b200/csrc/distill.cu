@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kDistillThreads) distill_grad_kernel(const T* 
 // turn: a CTA may be a row ahead of another, never two).  A barrier of the cluster would also wait until the gradients that
 // the threads have stored are visible, which is several microseconds.
 //
-// What bounds it is issue (46 % of the cycles) and the chain of a row, copy to exchange to gradient, more than memory (53 %);
+// What bounds it is issue (half of the cycles) and the chain of a row, copy to exchange to gradient, as much as memory (55 %);
 // so the rows are visited in an order that mixes neighbours: those without a teacher, which are only cleared, come in long runs
 // (image tokens), and their stores run beside the others' arithmetic this way.  The case of launch_mode: 234 us in order, 216
 // mixed, both before the second powers' squarings were unrolled; with 256 threads instead of 128, 242 and 232.

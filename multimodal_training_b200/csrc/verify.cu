@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(Verify v) {
 // ----------------------------------------------------------------------------
 // Sequences.  The first CTA of a sequence's cluster writes its answers.  A rejected draft costs four fp64 powers a column: two
 // for the rows' sums, two for max(p - q, 0); an accepted one nothing, and the row behind the last one power.  Those powers
-// bound it: 64 us for the 48 sequences above, 56 % of the issue slots.  A sequence by itself is a chain of barriers: 22 us with
+// bound it: 64 us for the 48 sequences above, half of the issue slots and a third of the fp64 pipe.  A sequence by itself is a chain of barriers: 22 us with
 // its rows.  256 threads of 128 registers: 87 us with the rows, 512 of 64: 95, three CTAs of 256 an SM: 97.  Half as many CTAs
 // again as fill the SMs once: 107 instead of 95, both with 512 threads.
 // ----------------------------------------------------------------------------
