@@ -17,6 +17,7 @@
 // equal logits that come later do not reach it.
 //
 // Few rows are cut into runs of columns, one for each CTA of a cluster; the first CTA ranks the others' lists.
+#include "key_range.h"
 #include "vocab_rows.cuh"
 
 namespace {
@@ -27,7 +28,7 @@ constexpr int kTopMax = 256;          // largest k
 constexpr int kTopSets = 4;           // vectors that a thread loads ahead: one of each set
 constexpr int kTopFull = 1024;        // candidates from which on the list is cut
 constexpr int kTopCluster = 8;        // most CTAs of a row; their lists fit one list: 8 * 256 = 2048
-constexpr int kTopBins = 256;
+constexpr int kTopBins = KeyRange::kBins;
 constexpr int kTopEdge = 16;          // elements outside whole vectors, at most 7 at each end
 
 template <int kTopThreads>
@@ -121,32 +122,31 @@ MMT_DEVICE void rank_list(TopShared<kTopThreads>& s, int n, int k, int shift, ui
     uint32_t most = 0;
     for (int i = tid; i < n; i += kTopThreads) most = max(most, (uint32_t)(s.list[i] >> shift) & 0xffffu);
     most = range_of_block<kTopThreads>(s, most, most).y;
-    // keys in [low, low + bins) compete for `need` places; those above have theirs
-    u64 low = (u64)bound << shift;
-    int wide = shift + 32 - __clz((most - bound) / kTopBins), need = k, sure = 0;
+    // keys that the range holds compete for `need` places; those above have theirs
+    KeyRange range(bound, most, shift);
+    int need = k, sure = 0;
     for (;;) {
       for (int b = tid; b < kTopBins; b += kTopThreads) s.hist[b] = 0;
       if (tid == 0) s.kept = 0;
       __syncthreads();
       for (int i = tid; i < n; i += kTopThreads) {
         const u64 key = s.list[i];
-        if (key >= low && (key - low) >> wide < kTopBins) atomicAdd(&s.hist[(int)((key - low) >> wide)], 1);
+        if (range.holds(key)) atomicAdd(&s.hist[range.bin(key)], 1);
       }
       __syncthreads();
       find_digit(s, need);
       __syncthreads();
-      low += (u64)s.digit << wide;
+      range.raise(s.digit);
       sure += need - s.need;
       need = s.need;
       const int left = sure + s.count;
-      if (left <= k + 64 || wide == 0) break;
-      wide = max(wide - 8, 0);
+      if (left <= k + 64 || !range.narrow()) break;
       __syncthreads();                            // all have read what find_digit found
     }
     for (int i0 = 0; i0 < n; i0 += kTopThreads) { // in place: what is written has been read
       const u64 key = i0 + tid < n ? s.list[i0 + tid] : 0;
       __syncthreads();
-      if (key != 0 && key >= low) s.list[atomicAdd(&s.kept, 1)] = key;
+      if (key != 0 && key >= range.low) s.list[atomicAdd(&s.kept, 1)] = key;
       __syncthreads();
     }
     n = s.kept;

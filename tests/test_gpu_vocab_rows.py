@@ -93,6 +93,38 @@ def test_top_logits_of_a_block_a_row(V, dtype, kind):
                            want_v.repeat(100, 1).view(torch.int16 if dtype == BF16 else torch.int32))
 
 
+def _tied_rows(V, dtype):
+    """Rows of which many logits share the k-th place, far below the largest one or as the largest one."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.full((8, V), -1.0)
+    x[1] = -0.5
+    for r, some in ((2, 20), (3, 40), (4, 100)):    # log-probabilities of a masked vocabulary
+        some = min(some, V)
+        x[r] = -INF
+        x[r, torch.randperm(V, generator=g)[:some]] = -0.3 - 5.7 * torch.rand(some, generator=g)
+    x[5] = 0.0                                      # few late positive logits
+    x[5, -min(100, V):] = 2.0 + 30 * torch.rand(min(100, V), generator=g)
+    x[6, ::2] = -2.0
+    x[7] = -1e4
+    x[7, V // 2] = 3.0
+    return x.to(dtype).cuda()
+
+
+@pytest.mark.parametrize("V", [130, 300, 1000, 2048, 5003, 30001, 152064])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("copies", [1, 80])
+def test_top_logits_of_rows_with_many_equal_ones(V, dtype, copies):
+    """With 8 rows they are cut over blocks, with 640 a block has a row, in the sizes that k and V ask for."""
+    F = _ops()
+    x = _tied_rows(V, dtype)
+    wide = x.repeat(copies, 1)
+    want_v, want_i = oracle.top(x, min(V, 256))
+    for k in sorted({min(V, k) for k in (40, 64, 65, 100, 129, 130, 150, 191, 200, 230, 255, 256)}):
+        values, ids = F.top_logits(wide, k)
+        assert torch.equal(ids.cpu(), want_i[:, :k].repeat(copies, 1)), k
+        assert torch.equal(values.cpu(), want_v[:, :k].repeat(copies, 1)), k
+
+
 def test_rows_behind_two_to_the_31_elements():
     F = _ops()
     ld, V = 1_100_000_003, 1001
