@@ -44,11 +44,11 @@ struct DistillCall {
 };
 
 // Per row, in statistics of [kStats][rows], of this shard: m c and m c1, S and S1, (x - m) c1 of the label if it is here and
-// 1 then, sum of p (x - m) c and of p over the slots that are here.  Or parts of the row's loss, one from each CTA that has
-// worked on it, which start as zeros.
+// 1 then, sum of p (x - m) c and of p over the slots that are here; and the row's loss, for which further backward passes
+// leave the others as they are.  Or parts of the row's loss, one from each CTA that has worked on it, which start as zeros.
 constexpr int kMaxCluster = 8;
-enum { kTop, kTop1, kSum, kSum1, kLabel, kDot, kMass, kMine, kStats };
-static_assert(kStats == kMaxCluster, "the parts of a row's loss lie where its statistics do");
+enum { kTop, kTop1, kSum, kSum1, kLabel, kDot, kMass, kMine, kLoss, kStats };
+static_assert(kStats >= kMaxCluster, "the parts of a row's loss lie where its statistics do");
 
 // ----------------------------------------------------------------------------
 // Teacher's side: one warp per row.  An entry is absent if its id is negative or its logit -inf.  2048 rows of 64: 9 us, a
@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == kFewThreads ? 6 : 2)
 }
 
 // ----------------------------------------------------------------------------
-// Losses of the rows from their statistics, into the place of the first of them.
+// Losses of the rows from their statistics.
 // ----------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) distill_row_loss_kernel(DistillRows rows, DistillCall call, long n_rows,
                                                                double* stats) {
@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(256) distill_row_loss_kernel(DistillRows rows,
   }
   if ((mark & kLabelled) && w.labelled > 0.0)
     loss += w.labelled * kLn2 * (log2(stats[kSum1 * n_rows + r]) - stats[kLabel * n_rows + r]);
-  stats[r] = loss;
+  stats[kLoss * n_rows + r] = loss;
 }
 
 // The sum of n losses, always in the same order: one CTA, 4 us for 2048 rows of 8 parts.
@@ -891,8 +891,8 @@ int mmt_distill_loss(const MmtDistill* d, float* loss, void* stream) {
                                         rows_of(*d), call_of(*d), d->rows, d->stats);
     if (e) return e;
   }
-  return (int)launch_dependent(distill_loss_kernel, 1, kLossThreads, 0, VR_STREAM(stream), d->stats,
-                               d->rows * (d->parts ? d->parts : 1), loss);
+  return (int)launch_dependent(distill_loss_kernel, 1, kLossThreads, 0, VR_STREAM(stream),
+                               d->parts ? d->stats : d->stats + kLoss * d->rows, d->rows * (d->parts ? d->parts : 1), loss);
 }
 
 // The sum of the runs of a product whose K was cut (mmt_gemm_bf16_split), as [rows, cols] bf16.

@@ -180,7 +180,7 @@ class _Distill:
         lib = nv.lib()
         per, n_stats = lib.mmt_distill_count_rows(), lib.mmt_distill_stats_count()
         n_counts = (rows + per - 1) // per
-        # one workspace, 8-byte words first: statistics, info, pairs of counts, tickets, ids and probabilities, marks
+        # one workspace, 16-byte words first: info, statistics, pairs of counts, tickets, ids and probabilities, marks
         n_slots = rows * (K + 1)
         self.n_stats = n_stats * rows
         at_counts = self.n_stats + 2 * rows
@@ -188,7 +188,7 @@ class _Distill:
         self.work = torch.empty(words + n_slots + (rows + 1) // 2, device=teacher_ids.device, dtype=torch.float64)
         at = self.work.data_ptr()
         w = self.words = _DistillWords(rows=rows, vocab_lo=vocab_lo, temperature=temperature, share=share, V=V, K=K,
-                                       is_f32=int(is_f32), stats=at, info=at + 8 * self.n_stats, counts=at + 8 * at_counts,
+                                       is_f32=int(is_f32), info=at, stats=at + 16 * rows, counts=at + 8 * at_counts,
                                        ticket=at + 8 * (words - 1), slot_id=at + 8 * words,
                                        slot_p=at + 8 * words + 4 * n_slots, mark=at + 8 * (words + n_slots))
         if rows:
@@ -198,7 +198,8 @@ class _Distill:
 
     @property
     def stats(self) -> torch.Tensor:
-        return self.work[:self.n_stats].view(nv.lib().mmt_distill_stats_count(), self.words.rows)
+        rows = self.words.rows
+        return self.work[2 * rows:2 * rows + self.n_stats].view(nv.lib().mmt_distill_stats_count(), rows)
 
     def _rows(self, logits, src, cnt):
         w = self.words
@@ -217,7 +218,7 @@ class _Distill:
         top = stats[:2, lo:hi].contiguous()
         mine = top.clone()
         F._all_reduce(top, torch.distributed.ReduceOp.MAX, group)
-        rest = stats[2:, lo:hi].contiguous()
+        rest = stats[2:8, lo:hi].contiguous()
         sums, label, dot, mass, has_label = rest[:2], rest[2], rest[3], rest[4], rest[5]
         # from below this shard's largest logit to below the whole vocabulary's; a shard of nothing but -inf has a sum of
         # zero, which stays
@@ -227,7 +228,7 @@ class _Distill:
         dot.add_(torch.where(mass > 0, mass * down[0], 0.0))
         F._all_reduce(rest, torch.distributed.ReduceOp.SUM, group)
         stats[:2, lo:hi] = top
-        stats[2:, lo:hi] = rest
+        stats[2:8, lo:hi] = rest
 
     def _out(self, out, dloss=None) -> None:
         w = self.words

@@ -306,6 +306,81 @@ def test_distillation_of_vocabulary_shards(monkeypatch, dtype, temperature, shar
           dtype)
 
 
+def _group_of(monkeypatch, world, all_reduce):
+    """A process group of `world` ranks of which this process is one."""
+    from multimodal_training_b200.ops import vocab_rows
+    monkeypatch.setattr(vocab_rows, "_multi", lambda group: group is not None)
+    monkeypatch.setattr(torch.distributed, "get_world_size", lambda group=None: world)
+    monkeypatch.setattr(_ops(), "_all_reduce", all_reduce)
+    return object()
+
+
+@pytest.mark.parametrize("temperature,share", [(1.0, 0.0), (2.0, 0.3), (0.5, 1.0)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_repeated_backward_passes_of_vocabulary_shards(monkeypatch, dtype, temperature, share):
+    """The loss is there before the gradient is formed again."""
+    import threading
+    T, V, K, world = 12, 1000, 6, 2
+    x, ids, teacher, labels = _batch(T, V, K, dtype)
+    meet, given, rank_of = threading.Barrier(world, timeout=60), [None] * world, threading.local()
+
+    def all_reduce(t, op, group):
+        given[rank_of.rank] = t.clone()
+        meet.wait()
+        both = torch.stack(given)
+        meet.wait()
+        t.copy_(both.amax(0) if op == torch.distributed.ReduceOp.MAX else both.sum(0))
+
+    group, out = _group_of(monkeypatch, world, all_reduce), [None] * world
+    factors = (1.0, 0.25, 3.0)
+
+    def rank(r):
+        rank_of.rank = r
+        lo = r * (V // world)
+        mine = x[:, lo:lo + V // world].detach().requires_grad_()
+        loss = _ops().distillation_loss(mine, ids, teacher, temperature=temperature, labels=labels, label_weight=share,
+                                        vocab_lo=lo, group=group)
+        out[r] = loss.detach(), [torch.autograd.grad(loss, mine, torch.tensor(f, device="cuda"), retain_graph=True)[0]
+                                 for f in factors]
+
+    threads = [threading.Thread(target=rank, args=(r,)) for r in range(world)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    want, dx, size = oracle.distill(x, ids, teacher, temperature, labels, share)
+    for i, f in enumerate(factors):
+        _near(out[0][0], torch.cat([g[i] for _, g in out], 1), want, f * dx, f * size, temperature, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_captured_backward_pass_of_a_vocabulary_shard(monkeypatch, dtype):
+    """The other rank's half of the vocabulary has no mass, so that this one's answer is the whole one."""
+    T, V, K = 12, 1000, 6
+    group = _group_of(monkeypatch, 2, lambda t, op, group: None)
+    x, ids, teacher, labels = _batch(T, V, K, dtype)
+    x.requires_grad_()
+
+    def step():
+        loss = _ops().distillation_loss(x, ids, teacher, temperature=2.0, labels=labels, label_weight=0.3, group=group)
+        return loss.detach(), torch.autograd.grad(loss * 0.5, x)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, grad = step()
+    for seed in (1, 2):
+        y = _batch(T, V, K, dtype, seed=seed)[0]
+        with torch.no_grad():
+            x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, dx, size = oracle.distill(y, ids, teacher, 2.0, labels, 0.3)
+        _near(loss, grad, want, 0.5 * dx, 0.5 * size, 2.0, dtype)
+
+
 def test_rows_that_all_weight_leaves_are_not_read():
     x, ids, teacher, labels = _batch(8, 500, 4, BF16)
     labels[:] = torch.tensor([3, -100] * 4)
