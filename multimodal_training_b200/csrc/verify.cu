@@ -210,8 +210,10 @@ struct Powers16 {
   MMT_DEVICE Powers16(double scale_, double largest_)
       : scale(scale_), shift(kMagic - rint(largest_ * scale_)), largest(largest_),
         least((float)(largest_ - 16.0 * 900.0 / scale_)) {}
-  // Whether the largest logit is too far from zero for a whole number beside kMagic; such a row takes the long way.
-  MMT_DEVICE bool far() const { return fabs(largest) * scale > 0x1p45; }
+  // Whether the largest logit is too far from zero for `least`, whose rounding to fp32 moves it by 2^-24 of that distance: up to
+  // here that is 64 of the 900 powers of two, and what is left is between 2^-964, where the exponent still fits, and 2^-836,
+  // which is nothing.  Rows further out take the long way.  (Beside kMagic a whole number has room up to 2^51.)
+  MMT_DEVICE bool far() const { return fabs(largest) * scale > 0x1p34; }
   MMT_DEVICE double any(float x, const double* table) const {
     return far() ? exp2(((double)x - largest) * (scale / 16.0)) : of(x, table);
   }

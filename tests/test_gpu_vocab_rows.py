@@ -695,6 +695,37 @@ def test_verification_of_rows_far_from_zero(dtype, temperature):
     _same(got, oracle.verify(target, ids, draft, u, temperature))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("temperature", [1.0, 2.0 ** -20])
+@pytest.mark.parametrize("drafter", [False, True])
+def test_verification_at_every_distance_from_zero(dtype, sign, temperature, drafter):
+    """Largest logits of 2^20 to 2^60 temperatures; logits a few steps of their type below, at half or twice the distance from
+    zero, at zero, without mass."""
+    F = _ops()
+    V, exponents = 1501, range(20, 61)
+    g = torch.Generator().manual_seed(8)
+    n = len(exponents)
+    top = torch.tensor([sign * 2.0 ** e * temperature for e in exponents]).to(dtype)
+    below = [top]
+    for _ in range(3):
+        bits = below[-1].view(torch.int16 if dtype == BF16 else torch.int32)
+        below.append((bits - int(sign)).view(dtype))
+    assert all((b < a).all() for a, b in zip(below, below[1:]))
+    far = torch.full_like(top, -INF)
+    choice = torch.stack([*below, top * (0.5 if sign > 0 else 2), -0.25 * top if sign > 0 else 3 * top, far])   # [7, n]
+    pick = torch.randint(1, 7, (n, 3, V), generator=g)
+    pick[torch.rand(n, 3, V, generator=g) < 0.01] = 0
+    pick[:, :, 700] = 0
+    rows = choice.T[:, None].expand(n, 3, 7).gather(2, pick).cuda()
+    target, draft = rows[:, :2], rows[:, 2:] if drafter else None
+    ids = torch.randint(0, V, (n, 1), generator=g)
+    ids[::2] = 700
+    ids, u = ids.cuda(), torch.rand(n, 2, generator=g).cuda()
+    got = F.verify_drafts(target, ids, draft, u, temperature=temperature)
+    _same(got, oracle.verify(target, ids, draft, u, temperature))
+
+
 def test_rows_behind_a_shorter_draft_are_not_read():
     F = _ops()
     target, ids, draft, u = _drafts(3, 4, 2000, BF16)
