@@ -9,8 +9,8 @@
 //
 // A drawn token depends on a sum over the whole vocabulary that may end next to a border: an error e of the cumulative
 // weights gives another token with probability 2 V e.  So the row that is drawn from is weighed in fp64.  The normalisers of
-// all rows, one pass over memory, are fp32 sums; their error is below 2^-15 (a thread adds up to 300 terms one by one), so a
-// draft whose acceptance that could change has its two rows summed again in fp64.
+// all rows, one pass over memory, are fp32 sums of a bounded error (sum_error), so a draft whose acceptance that could change
+// has its two rows summed again in fp64.
 #include "vocab_rows.cuh"
 
 namespace {
@@ -59,6 +59,15 @@ MMT_DEVICE Row<T> draft_row(const Verify& v, int b, int i) {
 }
 // fp32 exponents are (x - m) c, as in the sums of csrc/distill.cu.
 MMT_DEVICE float scale_of(const Verify& v) { return (float)(kLog2e * v.inv_temperature); }
+
+// Bound on the relative error of a row's fp32 sum, in which a thread adds kRowAhead vectors a step.  In units of 2^-24: a step
+// may scale what there is by another power (four for ex2.approx, one for the product) and adds to it (one); besides those a
+// term's power (four) and its exponent, whose three roundings count in proportion to it, 20.8 on the average of a
+// distribution over 2^30 ids; 16 additions of a step and 15 of the threads, warps and their scales.
+MMT_DEVICE double sum_error(const Verify& v) {
+  const int vec = v.is_f32 ? 4 : 8, per = (v.V / vec + v.splits) / v.splits + 1;
+  return (6.0 * ((per - 1) / (kRowAhead * kRowThreads) + 1) + 100.0) * 0x1p-24;
+}
 
 // ----------------------------------------------------------------------------
 // Rows: (largest logit, sum), or the key of the largest logit, of each part of a row.  One pass over memory: 139 MB (the rows
@@ -312,6 +321,8 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(Verify v) 
   cluster_barrier();                               // every CTA has started: its shared memory may be written
   int turn = 0;
   const double scale = 16.0 * kLog2e * v.inv_temperature;      // of Powers16
+  // what p / q may be off by, twice over: 2^-13 up to 550,000 columns (270,000 in fp32) in one part
+  const double margin = 1.0 + fmax(4.0 * sum_error(v), 0x1p-13);
 
   // largest logit and normaliser of a row, from its parts; by a warp
   const float c = scale_of(v);
@@ -399,8 +410,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(Verify v) 
         const double p = known ? share(xp, sp) : 0.0, q = !v.draft ? 1.0 : known ? share(xq, sq) : 0.0;
         const double uq = uniform(v, b, i) * q;
         prob = p > 0.0 ? (p >= q ? 1.f : (float)(p / q)) : p == 0.0 ? 0.f : NAN;
-        // both sums may be off by 2^-15
-        verdict = uq * (1.0 + 0x1p-13) < p ? kStands : uq < p * (1.0 + 0x1p-13) && p > 0.0 ? kHangs : kFalls;
+        verdict = uq * margin < p ? kStands : uq < p * margin && p > 0.0 ? kHangs : kFalls;
         if (lane == 0) {
           s.logits[j] = make_float2(xp, xq);
           s.largest[j] = make_float2((float)sp.x, (float)sq.x);

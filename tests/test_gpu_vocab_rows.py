@@ -726,6 +726,22 @@ def test_verification_at_every_distance_from_zero(dtype, sign, temperature, draf
     _same(got, oracle.verify(target, ids, draft, u, temperature))
 
 
+def test_acceptance_where_sums_of_fp32_are_long():
+    """So many rows that none is cut: a thread adds its part of 2^25 columns in 8192 steps, each of them lost beside a one."""
+    F = _ops()
+    B, V = 600, 2 ** 25
+    row = torch.full((V,), -27.01 * math.log(2.0), device="cuda")
+    row[:1024:4] = 0.0                              # one for each of 256 threads
+    total = 256.0 + (V - 256) * 2.0 ** -27.01       # a fp32 sum may be off by half of the second term, 2^-11 of all
+    u = torch.zeros(B, 2, dtype=torch.float64)
+    u[:, 1] = 0.5
+    u[0, 0] = (1.0 + 1e-4) / total                  # not accepted, by less than the sum's error
+    got = F.verify_drafts(row.expand(B, 2, V), torch.zeros(B, 1, dtype=torch.int64, device="cuda"), None, u.cuda())
+    assert got.accepted.tolist() == [0] + [1] * (B - 1)
+    # half of the mass, with and without the first id, ends behind the ones at 0, 4, ... 508
+    assert got.tokens[0].tolist() == [512, -1] and (got.tokens[1:].cpu() == torch.tensor([0, 512])).all()
+
+
 def test_rows_behind_a_shorter_draft_are_not_read():
     F = _ops()
     target, ids, draft, u = _drafts(3, 4, 2000, BF16)
