@@ -346,6 +346,13 @@ def _check_distill(shape, device, teacher_ids, teacher_logits, temperature, labe
     return ids, _rows(teacher_logits), labels
 
 
+def _check_shard(V, vocab_lo, group):
+    """The shard's place in a vocabulary of as many equal ones as the group has ranks."""
+    world = torch.distributed.get_world_size(group) if _multi(group) else 1
+    if not 0 <= vocab_lo <= V * (world - 1):
+        raise ValueError(f"vocab_lo = {vocab_lo}: {world} shard(s) of {V} ids start between 0 and {V * (world - 1)}")
+
+
 def _distill_reference(logits, ids, teacher, labels, temperature, share, vocab_lo, group):
     """Plain PyTorch, differentiable; fp32 or the logits' wider type."""
     from ..parallel.comm import all_reduce_sum_autograd
@@ -407,10 +414,12 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
 
     The result is an fp32 scalar, differentiable with respect to ``logits`` only.  On the GPU an id outside the vocabulary
     is left out and reported through the device error word.  With a group, ``logits`` are this rank's shard of the
-    vocabulary, starting at ``vocab_lo``, as in :func:`.functional.lm_head_cross_entropy`.
+    vocabulary, one of as many equal ones as there are ranks, starting at ``vocab_lo``, as in
+    :func:`.functional.lm_head_cross_entropy`; without one, ``vocab_lo`` is 0.
     """
     V = _vocab(logits)
     _floating(logits, "logits")
+    _check_shard(V, vocab_lo, group)
     gpu = _on_gpu(logits, teacher_ids, teacher_logits, labels)
     ids, teacher, labels = _check_distill(logits.shape[:-1], logits.device, teacher_ids, teacher_logits, temperature, labels,
                                           label_weight)
@@ -542,6 +551,7 @@ def lm_head_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids
     if hidden.dtype != weight.dtype:
         raise TypeError(f"hidden is {hidden.dtype}, weight {weight.dtype}")
     _floating(hidden, "hidden")
+    _check_shard(weight.shape[0], vocab_lo, group)
     from . import functional as F
     gpu = _on_gpu(hidden, weight, teacher_ids, teacher_logits, labels)
     ids, teacher, labels = _check_distill(hidden.shape[:1], hidden.device, teacher_ids, teacher_logits, temperature, labels,

@@ -159,6 +159,30 @@ def test_distillation_refusals():
         F.lm_head_distillation(h, w.double(), ids, teacher)
 
 
+def test_a_shard_of_the_vocabulary_needs_its_group():
+    """Ids are those of the whole vocabulary: without the other ranks there is none that starts behind its first id."""
+    x, ids, teacher, _ = _batch(4, 24, 3)
+    h, w = torch.randn(4, 6), torch.randn(24, 6)
+    for lo in (1, 24, -1):
+        with pytest.raises(ValueError, match="vocab_lo"):
+            F.distillation_loss(x, ids, teacher, vocab_lo=lo)
+        with pytest.raises(ValueError, match="vocab_lo"):
+            F.lm_head_distillation(h, w, ids, teacher, vocab_lo=lo)
+
+
+def _shard_worker(rank, world, lo):
+    import torch.distributed as dist
+    x, ids, teacher, _ = _batch(4, 24, 3)
+    with pytest.raises(ValueError, match="vocab_lo"):
+        F.distillation_loss(x, ids, teacher, vocab_lo=lo, group=dist.group.WORLD)
+    return True
+
+
+@pytest.mark.parametrize("lo", [-1, 25])
+def test_a_shard_lies_in_the_vocabulary(tmp_path, lo):
+    assert run_ranks(_shard_worker, 2, tmp_path, lo) == [True, True]
+
+
 def test_head_and_logits_agree():
     x, ids, teacher, labels = _batch(9, 24, 5)
     h = torch.randn(9, 8, dtype=torch.float64, requires_grad=True)
