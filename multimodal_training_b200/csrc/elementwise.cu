@@ -1002,6 +1002,7 @@ int mmt_gather_rows(const void* src, const long* idx, void* dst, long rows, int 
                     long dst_ld, void* stream) {
   if (cols % 8 || src_ld % 8 || dst_ld % 8) return -2;
   if (rows == 0) return 0;
+  if ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) & 15) return -3;
   launch_dependent(gather_rows_kernel, (unsigned)((rows + 7) / 8), 256, 0, ST(stream),
                      CBF(src), idx, BF(dst), rows, cols, lo, hi,
                                                                         src_ld, dst_ld);

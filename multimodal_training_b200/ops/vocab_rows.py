@@ -560,9 +560,13 @@ def lm_head_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids
         logits = torch.nn.functional.linear(hidden, weight)
         return _distill_reference(logits, ids, teacher, labels, temperature, label_weight, vocab_lo, group)
     F._native(hidden)
-    if hidden.shape[1] % 8 or weight.shape[0] % 8 or not weight.is_contiguous():
-        raise ValueError(f"the sm_100a path needs a contiguous weight of multiples of 8, got {tuple(weight.shape)}")
-    return _LMHeadDistillFn.apply(F._c(hidden), weight, ids, teacher, labels, float(temperature), float(label_weight),
+    if hidden.shape[1] % 8 or weight.shape[0] % 8 or not weight.is_contiguous() or weight.data_ptr() % 16:
+        raise ValueError(f"the sm_100a path needs a contiguous weight of multiples of 8 that starts at a multiple of 16 bytes, "
+                         f"got {tuple(weight.shape)}")
+    hidden = F._c(hidden)
+    if hidden.data_ptr() % 16:                     # rows are read in 16-byte vectors
+        hidden = hidden.clone()
+    return _LMHeadDistillFn.apply(hidden, weight, ids, teacher, labels, float(temperature), float(label_weight),
                                   vocab_lo, group, chunk_rows)
 
 

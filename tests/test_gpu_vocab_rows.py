@@ -519,6 +519,25 @@ def test_head_of_hidden_states_that_are_not_numbers_where_nothing_is_taught():
         assert torch.equal(a, b)
 
 
+def test_head_of_hidden_states_at_any_address():
+    F = _ops()
+    T, H, V, K = 40, 64, 520, 4
+    g = torch.Generator().manual_seed(2)
+    h = torch.randn(T, H, generator=g).cuda().bfloat16()
+    w = torch.randn(V, H, generator=g).cuda().bfloat16()
+    _, ids, teacher, _ = _batch(T, V, K, BF16)
+    want = torch.autograd.grad(F.lm_head_distillation(h.requires_grad_(), w.requires_grad_(), ids, teacher), (h, w))
+    for off in (1, 3, 4):
+        there = torch.empty(T * H + off, device="cuda", dtype=BF16)[off:].view(T, H).copy_(h.detach()).requires_grad_()
+        assert there.data_ptr() % 16 and there.is_contiguous()
+        got = torch.autograd.grad(F.lm_head_distillation(there, w, ids, teacher), (there, w))
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    wide = torch.empty(V * H + 4, device="cuda", dtype=BF16)[4:].view(V, H).copy_(w.detach())
+    with pytest.raises(ValueError, match="16 bytes"):
+        F.lm_head_distillation(h, wide, ids, teacher)
+
+
 @pytest.mark.parametrize("temperature,share", [(1.0, 0.0), (4.0, 0.5), (0.5, 1.0)])
 def test_losses_without_gradients(temperature, share):
     F = _ops()

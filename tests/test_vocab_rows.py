@@ -183,6 +183,15 @@ def test_a_shard_lies_in_the_vocabulary(tmp_path, lo):
     assert run_ranks(_shard_worker, 2, tmp_path, lo) == [True, True]
 
 
+@pytest.mark.parametrize("src,dst", [(0x1008, 0x2000), (0x1002, 0x2000), (0x1000, 0x2004)])
+def test_rows_at_any_other_address_than_16_bytes_are_not_gathered(src, dst):
+    """The kernel reads and writes 16 bytes at a time; nothing is launched here."""
+    from multimodal_training_b200.ops import native as nv
+    if not nv.available():
+        pytest.skip("the kernel library is not built")
+    assert nv.lib().mmt_gather_rows(src, 0x3000, dst, 1, 8, 0, 1, 8, 8, None) == -3
+
+
 def test_head_and_logits_agree():
     x, ids, teacher, labels = _batch(9, 24, 5)
     h = torch.randn(9, 8, dtype=torch.float64, requires_grad=True)
