@@ -10,8 +10,10 @@
 //
 // Powers of two: with c = log2(e) / tau rounded to fp32 and m the row's largest logit, q_v = 2^((x_v - m) c) / S,
 // S = sum 2^((x - m) c).  Statistics and gradient use the same rounded c, which changes the temperature by 2^-24 and nothing
-// else; the difference is taken first, so any finite logits do, the lowest of their type among them.  S is summed in fp32
-// (relative error of a few 2^-24); everything that is K long is fp64.
+// else; the difference is taken first, so any finite logits do, the lowest of their type among them.  S is summed in fp32: a
+// power is off by 2^-22, and a thread adds its terms one by one, up to 200 of them where a cluster holds the row and V / 512
+// in the other kernels, each time 2^-24 at most (gradients of 777 x 50001 fp32 logits are off by less than 2^-22 of their
+// norm).  The teacher's probabilities are rounded to fp32; sums over the K of them are fp64.
 #include <numeric>
 
 #include "vocab_rows.cuh"
@@ -341,8 +343,8 @@ __global__ void __launch_bounds__(kDistillThreads) distill_grad_kernel(const T* 
 // once and its gradient written once.
 //
 // Second softmax (kMode): none, or that of temperature one for the labels.  If the temperature is two or four, its powers are
-// the first one's squared once or twice (c1 = tau c exactly; 200 us for the case of launch_mode,
-// 216 with a loop over the squarings).
+// the first one's squared once or twice (c1 = tau c exactly).  A whole step in the case of launch_mode: 193 us with one softmax,
+// 202 and 205 with two at temperatures of two and four, 250 at 0.7, 1.5 and 3, where a logit takes two powers.
 //
 // The parts travel as asynchronous stores that count themselves into an mbarrier of the CTA they go to (two of them, in
 // turn: a CTA may be a row ahead of another, never two).  A barrier of the cluster would also wait until the gradients that
@@ -801,16 +803,16 @@ int launch_held(MmtDistill& d, int C, int per, void* stream) {
   const int step = d.cnt ? 1 : mixing_step((int)d.places);
   return (int)launch_cluster(kernel, (unsigned)(clusters * C), kThreads, C, bytes, VR_STREAM(stream),
                              reinterpret_cast<const T*>(d.logits), d.ld, d.V, rows_of(d), call_of(d), d.rows,
-                             (int)d.places, step, d.src, d.cnt, d.stats, d.ticket, d.dloss, reinterpret_cast<O*>(d.out), d.out_ld,
-                             per, mmt_error_word());
+                             (int)d.places, step, d.src, d.cnt, d.stats, d.ticket, d.dloss, reinterpret_cast<O*>(d.out),
+                             d.out_ld, per, mmt_error_word());
 }
 template <typename T, typename O, int kMode>
 int launch_mode(MmtDistill& d, void* stream) {
   const long nv = row_vectors(d);
   // As few CTAs a row as hold it in 39 KB each, of which an SM has five (smaller runs: six); more where there are few rows.
-  // 2048 x 152064 bf16, half of the rows with a teacher, two softmaxes: 200 us in runs of 37 KB, 215 in runs of 75 KB with two
-  // CTAs an SM.  512 x 152064 fp32, which eight CTAs hold in 75 KB each: 108 us
-  // with 256 threads, 110 with 512.
+  // 2048 x 152064 bf16, half of the rows with a teacher, two softmaxes at a temperature of two: 200 us in runs of 37 KB, 215 in
+  // runs of 75 KB with two CTAs an SM.  512 x 152064 fp32, which eight CTAs hold in 75 KB each: 108 us with 256 threads, 110
+  // with 512.
   int C = 1;
   while (C < kMaxCluster && nv * 16 > (long)kHeldBytes * C) C *= 2;
   while (C < kMaxCluster && d.places * C * 2 <= 2 * mmt_sm_count() && nv > 512L * C) C *= 2;

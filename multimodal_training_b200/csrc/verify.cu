@@ -192,9 +192,9 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(Verify v) {
 // ----------------------------------------------------------------------------
 // Sequences.  The first CTA of a sequence's cluster writes its answers.  A rejected draft costs four fp64 powers a column: two
 // for the rows' sums, two for max(p - q, 0); an accepted one nothing, and the row behind the last one power.  Those powers
-// bound it: 64 us for the 48 sequences above, half of the issue slots and a third of the fp64 pipe.  A sequence by itself is a chain of barriers: 22 us with
-// its rows.  256 threads of 128 registers: 87 us with the rows, 512 of 64: 95, three CTAs of 256 an SM: 97.  Half as many CTAs
-// again as fill the SMs once: 107 instead of 95, both with 512 threads.
+// bound it: 64 us for the 48 sequences above, half of the issue slots and a third of the fp64 pipe.  A sequence by itself is a
+// chain of barriers: 22 us with its rows.  256 threads of 128 registers: 87 us with the rows, 512 of 64: 95, three CTAs of 256
+// an SM: 97.  Half as many CTAs again as fill the SMs once: 107 instead of 95, both with 512 threads.
 // ----------------------------------------------------------------------------
 constexpr int kChunk = 32;            // drafts that are looked at together
 enum Verdict { kStands, kHangs, kFalls };
@@ -331,7 +331,9 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(Verify v) 
     const float2 none = make_float2(-INFINITY, 0.f);
     const float2 x = lane < v.splits ? part[lane] : none, y = lane + 32 < v.splits ? part[lane + 32] : none;
     const float m = warp_top(fmaxf(x.x, y.x));
-    auto of = [&](float2 p) { return p.x == -INFINITY ? (double)p.y : (double)p.y * exp2(((double)p.x - (double)m) * (double)c); };
+    auto of = [&](float2 p) {
+      return p.x == -INFINITY ? (double)p.y : (double)p.y * exp2(((double)p.x - (double)m) * (double)c);
+    };
     return make_double2((double)m, warp_total_of(of(x) + of(y)));
   };
   // largest logit's id of a row without sampling; by a warp
@@ -555,7 +557,8 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(Verify v) 
 
 // Parts of a row: enough CTAs for eight an SM, as long as each thread has kRowAhead vectors.
 int splits_of(long rows, int V, int is_f32) {
-  const long most = V / (is_f32 ? 4 : 8) / (kRowAhead * kRowThreads), want = (8L * mmt_sm_count() + rows - 1) / (rows > 0 ? rows : 1);
+  const long most = V / (is_f32 ? 4 : 8) / (kRowAhead * kRowThreads);
+  const long want = (8L * mmt_sm_count() + rows - 1) / (rows > 0 ? rows : 1);
   const long n = want < most ? want : most;
   return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }

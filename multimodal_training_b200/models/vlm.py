@@ -161,9 +161,10 @@ class Qwen2_5_VLForConditionalGeneration(nn.Module):
                  eos_token_id: int | None = None, *, temperature: float = 0.0, generator: torch.Generator | None = None,
                  draft_model: "Qwen2_5_VLForConditionalGeneration | None" = None, draft_tokens: int = 4) -> torch.Tensor:
         """Continuation of ONE sample; returns the full id sequence [S + new].  Greedy, or drawn at ``temperature`` (random
-        numbers from ``generator``; image and video placeholders are not drawn).  A ``draft_model`` with the same vocabulary proposes up to ``draft_tokens`` tokens,
-        which one pass of this model checks (:func:`..ops.functional.verify_drafts`): the answer has the distribution that
-        it has without a draft model, and is the same when greedy, up to the rounding of logits in passes of another length."""
+        numbers from ``generator``, which is on the model's device; image and video placeholders are not drawn).  A
+        ``draft_model`` with the same vocabulary proposes up to ``draft_tokens`` tokens, which one pass of this model checks
+        (:func:`..ops.functional.verify_drafts`): the answer has the distribution that it has without a draft model, and is
+        the same when greedy, up to the rounding of logits in passes of another length."""
         if draft_model is not None or temperature != 0.0:
             return self._generate_checked(input_ids, pixel_values, image_grid_thw, max_new_tokens, eos_token_id, temperature,
                                           generator, draft_model, draft_tokens)

@@ -149,8 +149,8 @@ class _DistillWords(ctypes.Structure):
                 ("cnt", ctypes.c_void_p), ("slot_id", ctypes.c_void_p), ("slot_p", ctypes.c_void_p),
                 ("info", ctypes.c_void_p), ("mark", ctypes.c_void_p), ("counts", ctypes.c_void_p),
                 ("stats", ctypes.c_void_p), ("ticket", ctypes.c_void_p), ("dloss", ctypes.c_void_p),
-                ("temperature", ctypes.c_double), ("share", ctypes.c_double), ("V", ctypes.c_int), ("K", ctypes.c_int), ("is_f32", ctypes.c_int),
-                ("out_f32", ctypes.c_int), ("parts", ctypes.c_int)]
+                ("temperature", ctypes.c_double), ("share", ctypes.c_double), ("V", ctypes.c_int), ("K", ctypes.c_int),
+                ("is_f32", ctypes.c_int), ("out_f32", ctypes.c_int), ("parts", ctypes.c_int)]
 
 
 nv.declare("mmt_distill_bytes", nv.c_int, [])
@@ -269,8 +269,11 @@ def _captured_with_forward(ctx) -> None:
 
 class _DistillFn(torch.autograd.Function):
     """The gradient is written in forward, while the row's statistics are at hand, and handed over by the first backward
-    pass (times its ``dloss``, where that is not one).  Another backward pass, and one that is captured into a graph (a
-    replay would scale once more), form it again from the logits."""
+    pass (times its ``dloss``, where that is not one: a bf16 gradient is then rounded a second time, unless the factor is a
+    power of two).  Another backward pass, and one that is captured into a graph (a replay would scale once more), form it
+    again from the logits, with the factor in front of the one rounding.
+
+    2048 x 152064 bf16, two softmaxes: 202 us, 454 with a factor of 1/3."""
 
     @staticmethod
     def forward(ctx, logits, teacher_ids, teacher_logits, labels, temperature, share, vocab_lo, group):
@@ -413,7 +416,9 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     temperature one, mean over the rows whose label is not negative).
 
     The result is an fp32 scalar, differentiable with respect to ``logits`` only.  On the GPU an id outside the vocabulary
-    is left out and reported through the device error word.  With a group, ``logits`` are this rank's shard of the
+    is left out and reported through the device error word, sums over the vocabulary and the teacher's probabilities are
+    fp32, ``teacher_logits`` of other types than bf16 and fp32 are rounded to fp32, and a gradient in bf16 is rounded once
+    when it is formed and once more by a factor of the loss that is no power of two.  With a group, ``logits`` are this rank's shard of the
     vocabulary, one of as many equal ones as there are ranks, starting at ``vocab_lo``, as in
     :func:`.functional.lm_head_cross_entropy`; without one, ``vocab_lo`` is 0.
     """
@@ -450,8 +455,14 @@ def _head_pass(hidden, weight, teacher, temperature, share, vocab_lo, group, chu
 
     As in the head's cross-entropy, the logits of a chunk of rows and their gradient live in workspaces only, and rows
     without a teacher or label are left out of the products in groups of 16.  The logits stay fp32: rounded to bf16 they
-    would move a row's loss by 2^-9 of their size, where the divergence is what is left of numbers of that size.  Their
-    gradient is rounded to bf16 once, for the tensor cores."""
+    would move a row's loss by 2^-9 of their size, where the divergence is what is left of numbers of that size.  (They are
+    sums of the tensor cores, which round towards zero: 1e-6 of their size too small for each 1000 of H, and the loss off by
+    2e-7 to 4e-6 of itself, where fp32 sums that round to nearest leave about 1e-7.)
+
+    Their gradient is rounded to bf16 once, for the tensor cores, as in the head's cross-entropy.  The gradients of hidden
+    states and weight are then off by 0.0020 to 0.0033 of their norm, most where one teacher's logit or label is nearly all of
+    a row; of fp32 products 0.0017 is left by the rounding of the result.  The part that is lost could only be had by the two
+    products over again with what the rounding leaves."""
     from . import functional as F
     T, V = hidden.shape[0], weight.shape[0]
     dev = hidden.device
@@ -492,8 +503,9 @@ def _head_pass(hidden, weight, teacher, temperature, share, vocab_lo, group, chu
 
 
 class _LMHeadDistillFn(torch.autograd.Function):
-    """Both gradients are produced in forward and handed over by the first backward pass, times its ``dloss``; another
-    one runs the products again.  In a captured graph they stay as forward left them, for the next replay."""
+    """Both gradients are produced in forward and handed over by the first backward pass, times its ``dloss`` (which rounds
+    them once more, unless it is a power of two); another one runs the products again.  In a captured graph they stay as
+    forward left them, for the next replay."""
 
     @staticmethod
     def forward(ctx, hidden, weight, teacher_ids, teacher_logits, labels, *call):
@@ -541,8 +553,10 @@ def lm_head_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids
     """:func:`distillation_loss` of ``hidden @ weight^T`` without keeping the logits: ``hidden`` is [T, H], ``weight`` this
     rank's [V_local, H] shard of the head, teacher and labels are those of the T rows.
 
-    On the GPU path hidden states and weight are bf16, H and V_local multiples of 8, and the weight gradient assumes
-    ``dloss == 1`` when it is written into ``main_grad``, as in :func:`.functional.lm_head_cross_entropy`.
+    On the GPU path hidden states and weight are bf16, H and V_local multiples of 8, the weight starts at a multiple of 16
+    bytes, and its gradient assumes ``dloss == 1`` when it is written into ``main_grad``, as in
+    :func:`.functional.lm_head_cross_entropy`.  The workspaces hold ``chunk_rows`` rows of fp32 logits and of their gradient in
+    bf16: 6 bytes a logit, 3.7 GB for 4096 rows of 152064, three times what the cross-entropy takes.
     """
     if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
         raise ValueError(f"hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} must be [T, H] and [V, H]")
@@ -578,7 +592,8 @@ class Verified(NamedTuple):
 
     accepted: torch.Tensor       # [B] int64: drafted tokens that stand
     tokens: torch.Tensor         # [B, n + 1] int64: those, the token that follows them, then -1
-    accept_prob: torch.Tensor    # [B, n] fp32: min(1, p / q) of every drafted token, 0 behind a sequence's last
+    accept_prob: torch.Tensor    # [B, n] fp32: min(1, p / q) of every drafted token, 0 behind a sequence's last; on the
+    #                              GPU of fp32 sums over the vocabulary
 
 
 _VERIFY_WORDS = struct.Struct("@2P4l7Pd8i")
@@ -668,7 +683,8 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
     largest logit (lowest id among equals, NaN above everything), which is also the next token.
 
     A drafted id outside the vocabulary is rejected.  A target row that is no distribution (NaN, all -inf) accepts nothing
-    and draws -1.  Probabilities and their sums are fp64, so the token does not depend on how the vocabulary is cut.
+    and draws -1.  Acceptance and the drawn token are those of fp64 probabilities and sums, so they do not depend on how the
+    vocabulary is cut.
     """
     if target_logits.dim() != 3 or draft_ids.dim() != 2:
         raise ValueError(f"target_logits {tuple(target_logits.shape)} and draft_ids {tuple(draft_ids.shape)} must be "
